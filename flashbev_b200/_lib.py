@@ -15,7 +15,9 @@ DEPTH_GAUSSIAN, DEPTH_LAPLACE, DEPTH_CATEGORICAL, DEPTH_CATEGORICAL_LOGITS = 0, 
 ABI_VERSION = 2
 POOL_MEAN, POOL_SUM = 0, 1
 BWD_FEATS, BWD_DEPTH, BWD_LEGACY_DEPTH, BWD_DETERMINISTIC = 1, 2, 4, 8
-DEV_BAD_FEATURE_SIZE = 1
+DEV_BAD_FEATURE_SIZE, DEV_TIMEOUT = 1, 2
+POS_F32, POS_I32, POS_I64 = 0, 1, 2
+ROTARY_MAX_PAIRS = 128
 WORKSPACE_BYTES = 16
 STATIC_SCRATCH_BYTES = 16 << 20
 SORT_BUDGET_BYTES = 256 << 20
@@ -28,6 +30,10 @@ EXPORTS = (
     "fbev_debug_indices",
     "fbev_flash_bevpool", "fbev_flash_bevpool_grad", "fbev_projection_matrices", "fbev_pillar_pool",
     "fbev_strerror", "fbev_version", "fbev_source_hash",
+    # include/fbev_query.h
+    "fbev_cross_attention", "fbev_cross_attention_grad", "fbev_cross_attention_lse_count",
+    "fbev_cross_attention_workspace_bytes", "fbev_rotary_axes", "fbev_add_rms_norm", "fbev_add_rms_norm_e4m3",
+    "fbev_add_rms_norm_grad", "fbev_add_rms_norm_grad_workspace_bytes",
 )
 # ... and include/fbev_debug.h (experiment and test helpers)
 DEBUG_EXPORTS = ("fbev_set_tuning", "fbev_set_experiment", "fbev_probe_read")
@@ -65,6 +71,35 @@ class FbevProblem(ctypes.Structure):
         ("saved_state", ctypes.c_void_p),
         ("saved_state_bytes", ctypes.c_uint64),
         ("depth_stats", ctypes.c_void_p),
+    ]
+
+
+class FbevAttention(ctypes.Structure):
+    """Mirror of ``struct FbevAttention`` (include/fbev_query.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("Lq", ctypes.c_int32), ("Lk", ctypes.c_int32),
+        ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("q_shared", ctypes.c_int32),
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("mask_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("key_lengths", ctypes.c_void_p), ("key_mask", ctypes.c_void_p), ("status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class FbevRotary(ctypes.Structure):
+    """Mirror of ``struct FbevRotary`` (include/fbev_query.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("L", ctypes.c_int32), ("H", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("pairs", ctypes.c_int32), ("axes", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("pos_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64 * 3), ("pos_stride", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("pair_turns", ctypes.c_double * ROTARY_MAX_PAIRS), ("pair_axis", ctypes.c_uint8 * ROTARY_MAX_PAIRS),
     ]
 
 
@@ -124,6 +159,26 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
     lib.fbev_projection_matrices.restype = i32
     lib.fbev_pillar_pool.argtypes = [i32, i32] + [vp] * 9 + [i32] * 4 + [f32, i32, vp, vp]
     lib.fbev_pillar_pool.restype = i32
+    att, sz = ctypes.POINTER(FbevAttention), ctypes.c_size_t
+    lib.fbev_cross_attention.argtypes = [att, vp, vp, vp]
+    lib.fbev_cross_attention.restype = i32
+    lib.fbev_cross_attention_grad.argtypes = [att] + [vp] * 7
+    lib.fbev_cross_attention_grad.restype = i32
+    lib.fbev_cross_attention_lse_count.argtypes = [att]
+    lib.fbev_cross_attention_lse_count.restype = sz
+    lib.fbev_cross_attention_workspace_bytes.argtypes = [att, i32]
+    lib.fbev_cross_attention_workspace_bytes.restype = sz
+    lib.fbev_rotary_axes.argtypes = [ctypes.POINTER(FbevRotary), vp, vp]
+    lib.fbev_rotary_axes.restype = i32
+    ll = ctypes.c_longlong
+    lib.fbev_add_rms_norm.argtypes = [i32, ll, i32, f32] + [vp] * 7
+    lib.fbev_add_rms_norm.restype = i32
+    lib.fbev_add_rms_norm_e4m3.argtypes = [i32, ll, i32, f32] + [vp] * 7
+    lib.fbev_add_rms_norm_e4m3.restype = i32
+    lib.fbev_add_rms_norm_grad.argtypes = [i32, ll, i32] + [vp] * 8 + [sz, vp]
+    lib.fbev_add_rms_norm_grad.restype = i32
+    lib.fbev_add_rms_norm_grad_workspace_bytes.argtypes = [ll, i32, i32]
+    lib.fbev_add_rms_norm_grad_workspace_bytes.restype = sz
     lib.fbev_set_tuning.argtypes = [i32] * 5
     lib.fbev_set_tuning.restype = None
     lib.fbev_set_experiment.argtypes = [i32]

@@ -655,11 +655,6 @@ extern "C" {
 
 int fbev_version(void) { return FBEV_ABI_VERSION; }
 
-#ifndef FBEV_SOURCE_HASH
-#define FBEV_SOURCE_HASH "unknown"
-#endif
-const char* fbev_source_hash(void) { return FBEV_SOURCE_HASH; }
-
 const char* fbev_strerror(int status) {
   switch (status) {
     case FBEV_OK: return "ok";
