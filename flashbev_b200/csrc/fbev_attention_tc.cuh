@@ -1,0 +1,536 @@
+// Attention on the tensor cores, 16-bit types.
+//
+// Forward.  A block owns up to two tiles of 128 rows (rows as in fbev_attention.cuh: query and head of the group) of one
+// sample and key head, and a range of key tiles of 128.  Per row tile and key tile, base 2 and with c = scale * log2 e:
+//
+//   S = Q K^T             operands in shared memory, 128 x 128 float32 accumulator in tensor memory
+//   P = 2^(c S - m)       one thread per row: tensor memory -> registers -> 16 bits, written over S
+//   O += P V              P from tensor memory, V from shared memory (read across its rows), accumulator in tensor memory
+//
+// Roles: eight softmax warps (two groups of four, one per row tile), a warp that loads by TMA, a warp that issues the
+// matrix instructions, a warp that reads the key mask and clears values that may not be attended.  While one row tile is
+// in the hands of its softmax group the tensor cores work on the other.
+//
+// m is the row's running maximum, raised only when a tile exceeds it by more than 8: weights then stay below 2^8 (no loss
+// in either type, both sides of the quotient carry the same factor) and the output, which lives in tensor memory, is
+// rescaled in a few of the first tiles only.
+//
+// Few rows (one row tile): both groups take the same rows, one the even and one the odd key tiles, and join in shared
+// memory at the end.  Whenever the row tiles leave SMs without a block the key tiles are split over several blocks, which
+// leave normalised float32 outputs and their logarithmic sums for att_join_kernel.
+//
+// Tensor memory, columns: S/P of group 0 and 1 (128 each), O of group 0 and 1 (128 each).
+#pragma once
+#include "fbev_attention.cuh"
+#include "fbev_tc.cuh"
+
+namespace fbev {
+
+struct AttPlan {
+  int G, TL;           // heads of a group, queries in a row tile (TL * G <= 128 rows)
+  int row_tiles;       // of a (sample, key head)
+  int pair;            // one row tile, even and odd key tiles
+  int row_blocks;      // blocks along the rows
+  int splits, per_split;  // blocks along the keys and their key tiles
+};
+
+struct AttFwdArgs {
+  CUtensorMap q, k, v;
+  FbevAttention p;
+  AttPlan pl;
+  void* out;
+  float* lse;       // final statistics or null
+  float* part;      // [splits][B * Hkv][rows][D] with splits > 1
+  float* part_lse;  // [splits][B * Hkv][rows_padded]
+  float c;          // |scale| * log2 e
+};
+
+template <int NSUB>
+struct AttFwdShape {
+  static constexpr int kStages = NSUB == 1 ? 10 : 5;
+  static constexpr uint32_t kStageBytes = NSUB * kTileBytes;
+  static constexpr uint32_t kSmem = 2 * kStageBytes + kStages * kStageBytes + 1024;
+};
+
+constexpr int kMaskRing = 4;
+constexpr int kAttThreads = 384;
+
+// O and statistics of one row leave: rounded to T, or float32 with the base-2 logarithm of the sum for the join
+template <typename T>
+__device__ __forceinline__ void store_row16(T* dst, const float* o, float f, int n) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    if (i >= n) break;
+    uint4 w;
+    w.x = pack2<T>(o[i] * f, o[i + 1] * f);
+    w.y = pack2<T>(o[i + 2] * f, o[i + 3] * f);
+    w.z = pack2<T>(o[i + 4] * f, o[i + 5] * f);
+    w.w = pack2<T>(o[i + 6] * f, o[i + 7] * f);
+    *reinterpret_cast<uint4*>(dst + i) = w;
+  }
+}
+__device__ __forceinline__ void store_row32(float* dst, const float* o, float f, int n) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    if (i >= n) break;
+    *reinterpret_cast<float4*>(dst + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+  }
+}
+
+template <typename T, int NSUB>
+__global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_constant__ AttFwdArgs a) {
+  using Shape = AttFwdShape<NSUB>;
+  constexpr int kStages = Shape::kStages;
+  constexpr uint32_t kStageBytes = Shape::kStageBytes;
+  extern __shared__ unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2 * kStages + kStages + 1 + 2 + 2 + 2 + 2 * kMaskRing + 1];
+  __shared__ uint32_t s_mask[kMaskRing][4];
+  __shared__ float s_stat[2][128];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_bail;
+
+  const AttPlan& pl = a.pl;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // block -> (split, row block, sample, key head); row blocks of one key head are neighbours and share its keys in L2
+  int u = blockIdx.x;
+  const int split = u % pl.splits;
+  u /= pl.splits;
+  const int rb = u % pl.row_blocks;
+  const int bg = u / pl.row_blocks, b = bg / a.p.Hkv, g = bg % a.p.Hkv;
+  const int keys = att_keys(a.p, b);
+  const int t0 = split * pl.per_split;
+  int n = (keys + 127) / 128 - t0;  // key tiles of this block
+  n = n < 0 ? 0 : n > pl.per_split ? pl.per_split : n;
+  const bool pair = pl.pair != 0;
+  const int tiles = pair ? 1 : (pl.row_tiles - 2 * rb < 2 ? 1 : 2);  // row tiles of this block
+  const bool masked = a.p.key_mask != nullptr;
+  const long long rows = att_rows(a.p);
+  const int tile_rows = pl.TL * pl.G;
+
+  const uint32_t smem = (smem_addr(s_raw) + 1023) & ~1023u;
+  const uint32_t s_q = smem, s_ring = smem + 2 * kStageBytes;
+  const uint32_t bars = smem_addr(s_bar);
+  const auto full = [&](int s) { return bars + 8 * s; };
+  const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
+  const auto fixed = [&](int s) { return bars + 8 * (2 * kStages + s); };
+  const uint32_t q_full = bars + 8 * (3 * kStages);
+  const auto s_full = [&](int i) { return bars + 8 * (3 * kStages + 1 + i); };
+  const auto p_full = [&](int i) { return bars + 8 * (3 * kStages + 3 + i); };
+  const auto o_full = [&](int i) { return bars + 8 * (3 * kStages + 5 + i); };
+  const auto m_full = [&](int i) { return bars + 8 * (3 * kStages + 7 + i); };
+  const auto m_empty = [&](int i) { return bars + 8 * (3 * kStages + 7 + kMaskRing + i); };
+  const uint32_t drained = bars + 8 * (3 * kStages + 7 + 2 * kMaskRing);
+
+  // softmax warps with rows to work on: all four of a group, fewer when the only row tile is short
+  const long long left = rows - (long long)(pair ? 0 : 2 * rb) * tile_rows;
+  const int live_rows = pair ? (int)(left < tile_rows ? left : tile_rows) : 128;
+  const int live_warps = (live_rows + 31) / 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+      mbar_init(fixed(s), 1);
+    }
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full(i), 1);
+      mbar_init(p_full(i), live_warps);
+      mbar_init(o_full(i), 1);
+    }
+    for (int i = 0; i < kMaskRing; ++i) {
+      mbar_init(m_full(i), 1);
+      mbar_init(m_empty(i), pair ? live_warps : 4 * tiles);
+    }
+    mbar_init(drained, 1);
+    s_bail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) tmem_alloc<512>(&s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const Bail bail{&s_bail, a.p.status};
+  // a tile whose values have to be cleared in places: masked, or cut off by the sample's length inside the tensor
+  const auto needs_fix = [&](int t) { return masked || ((t0 + t + 1) * 128 > keys && keys < a.p.Lk); };
+
+  if (warp >= 8) {
+    set_registers_down<80>();
+    if (warp == 8 && lane == 0 && n > 0) {
+      // ---- loads -------------------------------------------------------------------------------------------------
+      tma_prefetch(&a.q);
+      tma_prefetch(&a.k);
+      tma_prefetch(&a.v);
+      mbar_expect(q_full, (uint32_t)(tiles * NSUB * tile_rows * 128));
+      for (int i = 0; i < tiles; ++i)
+        for (int x = 0; x < NSUB; ++x)
+          tma_load_5d(s_q + i * kStageBytes + x * kTileBytes, &a.q, q_full, 64 * x, 0, g, (2 * rb + i) * pl.TL, a.p.q_shared ? 0 : b);
+      int slot = 0;
+      bool ok = true;
+      const auto load = [&](const CUtensorMap* map, int t) {
+        const int s = slot % kStages;
+        if (ok && slot >= kStages) ok = mbar_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
+        if (!ok) return;
+        mbar_expect(full(s), kStageBytes);
+        for (int x = 0; x < NSUB; ++x)
+          tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, (t0 + t) * 128, b);
+        ++slot;
+      };
+      load(&a.k, 0);
+      if (pair && n > 1) load(&a.k, 1);
+      const int ahead = pair ? 2 : 1;
+      for (int t = 0; t < n && ok; ++t) {
+        load(&a.v, t);
+        if (t + ahead < n) load(&a.k, t + ahead);
+      }
+      if (!ok) {
+        // nothing may be left in flight when the block ends
+        mbar_wait(q_full, 0, bail);
+        for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) {
+          const long long begin = clock64();
+          while (!mbar_try(full(i % kStages), (i / kStages) & 1) && clock64() - begin < 1000000000ll) {
+          }
+        }
+      }
+    } else if (warp == 9 && lane == 0 && n > 0) {
+      // ---- matrix instructions -----------------------------------------------------------------------------------
+      const bool negative = a.p.scale < 0.0f;
+      const int ksteps = (a.p.D + 15) / 16;
+      const uint32_t i_s = umma_instr<T>(128, false, negative), i_o = umma_instr<T>(ksteps * 16, true, false);
+      uint32_t fix_parity = 0;
+      int slot = 0;
+      bool ok = mbar_wait(q_full, 0, bail);
+      const auto take = [&]() {  // next tile of the ring, as shared-memory address
+        const int s = slot % kStages;
+        ok = ok && mbar_wait(full(s), (slot / kStages) & 1, bail);
+        ++slot;
+        return s;
+      };
+      const auto scores = [&](int i, int s) {
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < NSUB; ++x) {
+          const uint64_t da = desc_k_major(s_q + (pair ? 0 : i) * kStageBytes + x * kTileBytes);
+          const uint64_t db = desc_k_major(s_ring + s * kStageBytes + x * kTileBytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (x * 4 + k < ksteps) umma_ss(tmem + 128 * i, da + 2 * k, db + 2 * k, i_s, x + k > 0);
+        }
+        umma_commit(s_full(i));
+      };
+      const auto values = [&](int i, int s, bool first) {
+        tc_fence_after();
+        const uint64_t db = desc_mn_major(s_ring + s * kStageBytes);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) umma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, db + 128 * k, i_o, !first || k > 0);
+      };
+      const auto fix_wait = [&](int t, int s) {
+        if (!needs_fix(t)) return;
+        ok = ok && mbar_wait(fixed(s), (fix_parity >> s) & 1, bail);
+        fix_parity ^= 1u << s;
+      };
+      if (pair) {
+        for (int t = 0; t < 2 && t < n && ok; ++t) {
+          const int s = take();
+          if (!ok) break;
+          scores(t, s);
+          umma_commit(empty(s));
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          const int i = t & 1, s = take();
+          fix_wait(t, s);
+          ok = ok && mbar_wait(p_full(i), (t >> 1) & 1, bail);
+          if (!ok) break;
+          values(i, s, t < 2);
+          umma_commit(empty(s));
+          if (t + 2 >= n) umma_commit(o_full(i));
+          if (t + 2 < n) {
+            const int sk = take();
+            if (!ok) break;
+            scores(i, sk);
+            umma_commit(empty(sk));
+          }
+        }
+      } else {
+        const int sk0 = take();
+        if (ok) {
+          for (int i = 0; i < tiles; ++i) scores(i, sk0);
+          umma_commit(empty(sk0));
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          const int s = take();
+          fix_wait(t, s);
+          int sk = 0;
+          for (int i = 0; i < tiles; ++i) {
+            ok = ok && mbar_wait(p_full(i), t & 1, bail);
+            if (!ok) break;
+            values(i, s, t == 0);
+            if (i == tiles - 1) umma_commit(empty(s));
+            if (t + 1 == n) {
+              umma_commit(o_full(i));
+              continue;
+            }
+            if (i == 0) sk = take();
+            if (!ok) break;
+            scores(i, sk);
+            if (i == tiles - 1) umma_commit(empty(sk));
+          }
+        }
+      }
+      if (!ok) {
+        umma_commit(drained);
+        const long long begin = clock64();
+        while (!mbar_try(drained, 0) && clock64() - begin < 1000000000ll) {
+        }
+      }
+    } else if (warp == 10 && n > 0 && (masked || keys < a.p.Lk)) {
+      // ---- key mask, values that may not be attended ---------------------------------------------------------------
+      const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
+      bool ok = true;
+      int slot = pair && n > 1 ? 2 : 1;  // ring slot of the values of tile t: the keys loaded ahead come before
+      const int ahead = pair ? 2 : 1;
+      for (int t = 0; t < n && ok; ++t) {
+        const int s = slot % kStages, round = slot / kStages;
+        slot += t + ahead < n ? 2 : 1;
+        if (!needs_fix(t)) continue;
+        uint32_t word[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = (t0 + t) * 128 + 32 * i + lane;
+          word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
+        }
+        if (masked) {
+          const int m = t % kMaskRing;
+          if (t >= kMaskRing) ok = mbar_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
+          ok = __all_sync(kFull, ok);
+          if (!ok) break;
+          if (lane < 4) s_mask[m][lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m_full(m));
+        }
+        ok = __all_sync(kFull, mbar_wait(full(s), round & 1, bail));
+        if (!ok) break;
+        if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
+          // a row's 128 bytes: eight lanes, four rows at a time (the swizzle permutes within the row, zeros do not care)
+          for (int r = lane >> 3; r < 128; r += 4) {
+            const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
+            if ((w >> (r & 31)) & 1) continue;
+            for (int x = 0; x < NSUB; ++x)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16),
+                           "r"(0u)
+                           : "memory");
+          }
+          fence_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(fixed(s));
+      }
+    }
+  } else {
+    // ---- softmax ---------------------------------------------------------------------------------------------------
+    set_registers_up<208>();
+    const int i = warp >> 2, w4 = warp & 3;
+    const int r = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)(w4 * 32) << 16);
+    const uint32_t t_s = lanes + 128 * i, t_o = lanes + 256 + 128 * i;
+    const int mine = pair ? (n - i + 1) / 2 : (i < tiles ? n : 0);  // key tiles of this group
+    const bool works = w4 < live_warps && (pair || i < tiles);
+    const int row_tile = pair ? 0 : 2 * rb + i;
+    const long long row = (long long)row_tile * tile_rows + r;
+    const bool live = works && r < tile_rows && row < rows;
+    const int d16 = (a.p.D + 15) / 16 * 16;
+    float m = -INFINITY, sum = 0.0f;
+    bool ok = true;
+    if (works) {
+      for (int j = 0; j < mine; ++j) {
+        const int t = pair ? 2 * j + i : j;
+        uint32_t word[4] = {kFull, kFull, kFull, kFull};
+        bool cut = false;
+        if (masked) {
+          const int mr = t % kMaskRing;
+          ok = __all_sync(kFull, mbar_wait(m_full(mr), (t / kMaskRing) & 1, bail));
+          if (!ok) break;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) word[x] = s_mask[mr][x];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m_empty(mr));
+          cut = (word[0] & word[1] & word[2] & word[3]) != kFull;
+        } else if ((t0 + t + 1) * 128 > keys) {
+          const int have = keys - (t0 + t) * 128;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
+          cut = true;
+        }
+        ok = __all_sync(kFull, mbar_wait(s_full(i), j & 1, bail));
+        if (!ok) break;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld32(t_s + 32 * x, s + 32 * x);
+        tmem_wait_ld();
+        if (cut) {
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (!((word[x / 32] >> (x % 32)) & 1)) s[x] = -INFINITY;
+        }
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int x = 4; x < 128; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
+        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c;
+        const bool raise = mt > m + 8.0f;
+        if (__any_sync(kFull, raise)) {
+          const float back = raise ? (m == -INFINITY ? 0.0f : exp2_fast(m - mt)) : 1.0f;
+          if (raise) m = mt;
+          sum *= back;
+          // the output so far is complete: its last instruction came before the one that S waited for
+          if (j > 0) {
+#pragma unroll 1
+            for (int x = 0; x < d16; x += 32) {
+              float o[32];
+              tmem_ld32(t_o + x, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] *= back;
+              tmem_st32(t_o + x, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : -m;
+        float2 part[4] = {};
+        uint32_t packed[64];
+#pragma unroll
+        for (int x = 0; x < 64; ++x) {
+          const float2 e = fma2(make_float2(s[2 * x], s[2 * x + 1]), make_float2(a.c, a.c), make_float2(off, off));
+          const float2 pr = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+          part[x & 3] = add2(part[x & 3], pr);
+          packed[x] = pack2<T>(pr.x, pr.y);
+        }
+        tmem_st32(t_s, packed);
+        tmem_st32(t_s + 32, packed + 32);
+        const float2 all = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+        sum += all.x + all.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(i));
+      }
+      if (ok && mine > 0) ok = __all_sync(kFull, mbar_wait(o_full(i), 0, bail));
+      // the second group is about to write over the ring: the first group's tiles must have been consumed too
+      if (ok && pair && i == 1 && mine > 0) ok = __all_sync(kFull, mbar_wait(o_full(0), 0, bail));
+      tc_fence_after();
+    }
+    // ---- output ------------------------------------------------------------------------------------------------------
+    if (pair && n > 1) {
+      // the second group's rows join the first's through shared memory; the ring is idle, all tiles are consumed
+      float* s_join = reinterpret_cast<float*>(s_raw + (s_ring - smem_addr(s_raw)));  // [d16][128]
+      if (i == 1 && works) {
+#pragma unroll 1
+        for (int x = 0; x < d16; x += 32) {
+          float o[32];
+          tmem_ld32(t_o + x, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int y = 0; y < 32; ++y) s_join[(x + y) * 128 + r] = o[y];
+        }
+        s_stat[0][r] = m;
+        s_stat[1][r] = sum;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (i == 0 || !pair) {
+      float f0 = 1.0f, f1 = 0.0f;
+      const bool joins = pair && n > 1;
+      if (joins && works) {
+        const float m1 = s_stat[0][r], sum1 = s_stat[1][r];
+        const float mm = fmaxf(m, m1);
+        f0 = m == -INFINITY ? 0.0f : exp2_fast(m - mm);
+        f1 = m1 == -INFINITY ? 0.0f : exp2_fast(m1 - mm);
+        sum = sum * f0 + sum1 * f1;
+        m = mm;
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const bool parted = pl.splits > 1;
+      const long long l = row / pl.G;
+      T* dst = reinterpret_cast<T*>(a.out) + (((long long)b * a.p.Lq + l) * a.p.Hq + g * pl.G + (int)(row - l * pl.G)) * a.p.D;
+      const long long at = (long long)split * a.p.B * a.p.Hkv + bg;
+      float* dpart = a.part + (at * rows + row) * a.p.D;
+      const float* s_join = reinterpret_cast<const float*>(s_raw + (s_ring - smem_addr(s_raw)));
+      if (works || n == 0) {
+#pragma unroll 1
+        for (int x = 0; x < d16; x += 32) {
+          float o[32];
+          if (mine > 0) {
+            tmem_ld32(t_o + x, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+          }
+          if (joins) {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = o[y] * f0 + s_join[(x + y) * 128 + r] * f1;
+          }
+          if (!live) continue;
+          if (parted)
+            store_row32(dpart + x, o, inv, a.p.D - x);
+          else
+            store_row16<T>(dst + x, o, inv, a.p.D - x);
+        }
+      }
+      if (live) {
+        if (parted)
+          a.part_lse[at * att_rows_padded(a.p) + row] = sum == 0.0f ? -INFINITY : m + log2f(sum);
+        else if (a.lse != nullptr)
+          a.lse[(long long)bg * att_rows_padded(a.p) + row] = sum == 0.0f ? INFINITY : m + log2f(sum);
+      }
+    }
+    tc_fence_before();
+  }
+  grid_dependency_trigger();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_free<512>(tmem);
+  }
+}
+
+// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s: a warp per row
+template <typename T>
+__global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ FbevAttention p, const float* __restrict__ part,
+                                                       const float* __restrict__ part_lse, int splits, T* __restrict__ out,
+                                                       float* __restrict__ lse) {
+  grid_dependency_wait();
+  const long long rows = att_rows(p), padded = att_rows_padded(p), heads = (long long)p.B * p.Hkv;
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (unit >= rows * heads) return;
+  const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
+  const long long bg = unit / rows, row = unit - bg * rows;
+  const float* pl = part_lse + bg * padded + row;
+  float top = -INFINITY;
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, pl[s * heads * padded]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+  float total = 0.0f, o[4] = {};
+  if (top != -INFINITY) {
+    for (int s = 0; s < splits; ++s) {
+      const float w = exp2_fast(pl[s * heads * padded] - top);
+      if (w == 0.0f) continue;
+      total += w;
+      const float* src = part + ((s * heads + bg) * rows + row) * p.D;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < p.D) o[i] = fmaf(w, src[lane + 32 * i], o[i]);
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const long long l = row / G;
+  const int b = (int)(bg / p.Hkv), h = (int)(bg % p.Hkv) * G + (int)(row - l * G);
+  T* dst = out + (((long long)b * p.Lq + l) * p.Hq + h) * p.D;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < p.D) dst[lane + 32 * i] = from_float<T>(o[i] * inv);
+  if (lse != nullptr && lane == 0) lse[bg * padded + row] = total == 0.0f ? INFINITY : top + log2f(total);
+}
+
+}  // namespace fbev

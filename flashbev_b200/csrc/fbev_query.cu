@@ -5,8 +5,12 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <initializer_list>
+
 #include "fbev_query.h"
 #include "fbev_attention.cuh"
+#include "fbev_attention_tc.cuh"
 #include "fbev_norm.cuh"
 #include "fbev_rotary.cuh"
 
@@ -38,8 +42,173 @@ static bool has_pointers(const FbevAttention* p) {
 
 static size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
 
+// ---- tensor-core path -------------------------------------------------------------------------------------------------
+
+constexpr int kSms = 148;
+
+static bool tma_operand(const void* ptr, const int64_t (&stride)[3], const int64_t (&size)[3], bool first_unused) {
+  if ((uintptr_t)ptr % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (size[i] > 1 && !(i == 0 && first_unused) && (stride[i] <= 0 || stride[i] % 8 != 0 || stride[i] >= (1ll << 38))) return false;
+  return true;
+}
+
+// 16-bit types whose rows TMA can address: heads of whole 16 bytes, strides of whole 16 bytes.  Everything else takes the
+// one-warp-per-row kernels.
+static bool on_tensor_cores(const FbevAttention& p) {
+  if (p.dtype == FBEV_F32 || p.D % 8 != 0 || p.Lk == 0 || p.Lq == 0 || p.B == 0 || p.Hq / p.Hkv > 128) return false;
+  return tma_operand(p.q, p.q_stride, {p.B, p.Lq, p.Hq}, p.q_shared != 0) &&
+         tma_operand(p.k, p.k_stride, {p.B, p.Lk, p.Hkv}, false) && tma_operand(p.v, p.v_stride, {p.B, p.Lk, p.Hkv}, false);
+}
+
+static AttPlan attention_plan(const FbevAttention& p) {
+  AttPlan pl{};
+  pl.G = p.Hq / p.Hkv;
+  pl.TL = 128 / pl.G;
+  pl.row_tiles = (p.Lq + pl.TL - 1) / pl.TL;
+  pl.pair = pl.row_tiles == 1;
+  pl.row_blocks = (pl.row_tiles + 1) / 2;
+  // split the keys when the blocks along rows, heads and samples leave SMs idle
+  const long long blocks = (long long)p.B * p.Hkv * pl.row_blocks;
+  const int key_tiles = (p.Lk + 127) / 128;
+  long long splits = blocks < kSms ? kSms / blocks : 1;
+  if (splits > key_tiles) splits = key_tiles;
+  pl.per_split = (int)((key_tiles + splits - 1) / splits);
+  pl.splits = (key_tiles + pl.per_split - 1) / pl.per_split;
+  return pl;
+}
+
+static size_t split_output_bytes(const FbevAttention& p, const AttPlan& pl) {
+  return round_up((size_t)pl.splits * p.B * p.Hkv * att_rows(p) * p.D * 4, 256);
+}
+static size_t forward_workspace(const FbevAttention& p) {
+  if (!on_tensor_cores(p)) return 0;
+  const AttPlan pl = attention_plan(p);
+  if (pl.splits == 1) return 0;
+  return split_output_bytes(p, pl) + round_up((size_t)pl.splits * p.B * p.Hkv * att_rows_padded(p) * 4, 256);
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// the driver's encoder, looked up once (the library does not link against the driver)
+static EncodeTiled encode_tiled() {
+  static std::atomic<void*> found{nullptr};
+  void* fn = found.load(std::memory_order_acquire);
+  if (fn == nullptr) {
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &res) != cudaSuccess ||
+        res != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    found.store(fn, std::memory_order_release);
+  }
+  return reinterpret_cast<EncodeTiled>(fn);
+}
+
+// 64 elements x rows of a [.., tokens, heads, D] tensor in 128-byte rows; a dimension of one has any stride
+static int encode_map(CUtensorMap* map, int dtype, int rank, const void* ptr, const long long* dims, const long long* strides,
+                      const int* box) {
+  const EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return FBEV_ERR_NO_DEVICE;
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    bx[i] = (cuuint32_t)box[i];
+    if (i > 0) st[i - 1] = dims[i] > 1 ? (cuuint64_t)strides[i] * 2 : 128;
+  }
+  const CUresult rc = fn(map, dtype == FBEV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                         const_cast<void*>(ptr), d, st, bx, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+// rows (query, head of the group): box of TL queries
+static int encode_rows(CUtensorMap* map, const FbevAttention& p, const AttPlan& pl, const void* ptr, const int64_t* stride,
+                       bool shared) {
+  const long long dims[5] = {p.D, pl.G, p.Hkv, p.Lq, shared ? 1 : p.B};
+  const long long strides[5] = {1, stride[2], pl.G * stride[2], stride[1], stride[0]};
+  const int box[5] = {64, pl.G, 1, pl.TL, 1};
+  return encode_map(map, p.dtype, 5, ptr, dims, strides, box);
+}
+static int encode_keys(CUtensorMap* map, const FbevAttention& p, const void* ptr, const int64_t* stride) {
+  const long long dims[4] = {p.D, p.Hkv, p.Lk, p.B};
+  const long long strides[4] = {1, stride[2], stride[1], stride[0]};
+  const int box[4] = {64, 1, 128, 1};
+  return encode_map(map, p.dtype, 4, ptr, dims, strides, box);
+}
+
+// dynamic shared memory above 48 KiB is granted once per kernel and device
+template <typename K>
+static int allow_smem(K* kernel, uint32_t bytes, std::atomic<uint64_t>& done) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return FBEV_ERR_NO_DEVICE;
+  }
+  if (done.load(std::memory_order_acquire) >> dev & 1) return FBEV_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return FBEV_ERR_NO_DEVICE;
+  }
+  done.fetch_or(1ull << dev, std::memory_order_release);
+  return FBEV_OK;
+}
+
+// a kernel that may be brought in while the one before it drains; it calls grid_dependency_wait() first
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_next(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+// c of the exponentials: a scale of zero still has to turn a masked score of -infinity into a weight of zero
+static float score_factor(const FbevAttention& p) {
+  const float c = (p.scale < 0.0f ? -p.scale : p.scale) * kLog2e;
+  return c < 1e-30f ? 1e-30f : c;
+}
+
+template <typename T, int NSUB>
+static int tensor_forward(const FbevAttention& p, T* out, float* lse, cudaStream_t st) {
+  static std::atomic<uint64_t> granted{0};
+  AttFwdArgs a;
+  a.p = p;
+  a.pl = attention_plan(p);
+  int rc = allow_smem(att_fwd_kernel<T, NSUB>, AttFwdShape<NSUB>::kSmem, granted);
+  if (rc == FBEV_OK) rc = encode_rows(&a.q, p, a.pl, p.q, p.q_stride, p.q_shared != 0);
+  if (rc == FBEV_OK) rc = encode_keys(&a.k, p, p.k, p.k_stride);
+  if (rc == FBEV_OK) rc = encode_keys(&a.v, p, p.v, p.v_stride);
+  if (rc != FBEV_OK) return rc;
+  a.out = out;
+  a.lse = lse;
+  a.c = score_factor(p);
+  a.part = reinterpret_cast<float*>(p.workspace);
+  a.part_lse = a.pl.splits > 1 ? reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + split_output_bytes(p, a.pl)) : nullptr;
+  const long long blocks = (long long)p.B * p.Hkv * a.pl.row_blocks * a.pl.splits;
+  att_fwd_kernel<T, NSUB><<<(unsigned)blocks, kAttThreads, AttFwdShape<NSUB>::kSmem, st>>>(a);
+  if (a.pl.splits > 1)
+    launch_next(att_join_kernel<T>, (unsigned)((att_rows(p) * p.B * p.Hkv + 3) / 4), 128, 0, st, p, (const float*)a.part,
+                (const float*)a.part_lse, a.pl.splits, out, lse);
+  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+
 template <typename T>
 static int attention_forward(const FbevAttention& p, T* out, float* lse, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (on_tensor_cores(p) && (uintptr_t)out % 16 == 0)
+      return p.D <= 64 ? tensor_forward<T, 1>(p, out, lse, st) : tensor_forward<T, 2>(p, out, lse, st);
+  }
   const long long units = att_rows(p) * p.B * p.Hkv;
   att_row_kernel<T><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(p, out, lse);
   return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
@@ -69,7 +238,7 @@ size_t fbev_cross_attention_lse_count(const FbevAttention* p) {
 
 size_t fbev_cross_attention_workspace_bytes(const FbevAttention* p, int backward) {
   if (check_attention(p) != FBEV_OK) return 0;
-  return backward ? round_up(fbev_cross_attention_lse_count(p) * 4, 256) : 0;
+  return backward ? round_up(fbev_cross_attention_lse_count(p) * 4, 256) : forward_workspace(*p);
 }
 
 static int check_workspace(const FbevAttention* p, int backward) {
