@@ -1,0 +1,477 @@
+// Gradients of attention on the tensor cores, 16-bit types.
+//
+// With the forward's statistics (lse, base 2) and delta = <out, grad_out> per row, and c = scale * log2 e:
+//
+//   P = 2^(c S - lse),  dP = dO V^T,  dS = P (dP - delta),
+//   dQ = scale dS K,    dK = scale dS^T Q,    dV = P^T dO
+//
+// Two kernels of one shape, so that each sum has one owner and no atomic orders it: a block keeps a tile X of 128 rows
+// and walks the tiles Y of the other side.
+//
+//   dQ:     X = (Q, dO) of a row tile,  Y = (K, V) of the key tiles:   S = X0 Y0^T, dP = X1 Y1^T, acc0 += dS Y0
+//   dK, dV: X = (K, V) of a key tile,   Y = (Q, dO) of the row tiles:  the same transposed, and acc1 += P^T Y1
+//
+// S and dP are formed twice that way, seven products instead of the least of five; in exchange nothing of dQ travels to
+// memory in float32 and the result is the same from run to run.
+//
+// A 128 x 128 tile of S is in the hands of eight warps, a thread has 64 columns of a row: tensor memory -> registers ->
+// P in 16 bits back over S (needed as an operand only for dV), then dP -> dS in 16 bits back over dP.  Each half of the
+// columns writes over its own half only.  While the warps form P of the next tile, the tensor cores run acc0 of this one
+// and dP of the next; while they form dS, acc1 and S of the next.
+//
+// Tensor memory, columns: S/P 0, dP/dS 128, acc0 256, acc1 384.
+#pragma once
+#include "fbev_attention_tc.cuh"
+#include "fbev_rotary.cuh"
+
+namespace fbev {
+
+struct AttGradPlan {
+  int G, TL, row_tiles, key_tiles;
+  int splits, per_split;  // blocks along Y and their tiles
+};
+
+struct AttGradArgs {
+  CUtensorMap x0, x1, y0, y1;
+  FbevAttention p;
+  AttGradPlan pl;
+  const float* nlse;    // -lse and -delta of every row, laid out by row tile: [B * Hkv][row_tiles][128], rows that are not
+  const float* ndelta;  // there have a weight of zero (-infinity) and no delta
+  void* g0;      // dQ, or dK
+  void* g1;      // dV
+  float* part0;  // float32 parts of g0 and g1 with splits > 1, unscaled
+  float* part1;
+  float c;
+};
+
+// two resident tiles and a ring of at least four: Y0 and Y1 of a tile are held while Y0 of the next is read
+template <int NSUB>
+struct AttGradShape {
+  static constexpr int kStages = NSUB == 1 ? 10 : 4;
+  static constexpr uint32_t kStageBytes = NSUB * kTileBytes;
+  static constexpr uint32_t kSmem = (2 + kStages) * kStageBytes + 1024;
+};
+
+template <typename T, int NSUB, bool KV>
+__global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_constant__ AttGradArgs a) {
+  using Shape = AttGradShape<NSUB>;
+  constexpr int kStages = Shape::kStages;
+  constexpr uint32_t kStageBytes = Shape::kStageBytes;
+  extern __shared__ unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t s_bar[3 * kStages + 7 + 2 * kMaskRing];
+  __shared__ uint32_t s_mask[kMaskRing][4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_bail;
+
+  const AttGradPlan& pl = a.pl;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int u = blockIdx.x;
+  const int split = u % pl.splits;
+  u /= pl.splits;
+  const int x_tiles = KV ? pl.key_tiles : pl.row_tiles;
+  const int xt = u % x_tiles, bg = u / x_tiles, b = bg / a.p.Hkv, g = bg % a.p.Hkv;
+  const int keys = att_keys(a.p, b);
+  const bool masked = a.p.key_mask != nullptr;
+  const long long rows = att_rows(a.p);
+  const int tile_rows = pl.TL * pl.G;
+  const int t0 = split * pl.per_split;
+  int n = (KV ? (xt * 128 < keys ? pl.row_tiles : 0) : (keys + 127) / 128) - t0;  // tiles Y of this block
+  n = n < 0 ? 0 : n > pl.per_split ? pl.per_split : n;
+
+  const uint32_t smem = (smem_addr(s_raw) + 1023) & ~1023u;
+  const uint32_t s_x = smem, s_ring = smem + 2 * kStageBytes;
+  const uint32_t bars = smem_addr(s_bar);
+  const auto full = [&](int s) { return bars + 8 * s; };
+  const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
+  const auto fixed = [&](int s) { return bars + 8 * (2 * kStages + s); };
+  const uint32_t x_full = bars + 8 * (3 * kStages), s_full = x_full + 8, p_done = x_full + 16, dp_full = x_full + 24,
+                 ds_done = x_full + 32, acc_full = x_full + 40, drained = x_full + 48;
+  const auto m_full = [&](int i) { return drained + 8 + 8 * i; };
+  const auto m_empty = [&](int i) { return drained + 8 + 8 * (kMaskRing + i); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+      mbar_init(fixed(s), 1);
+    }
+    mbar_init(x_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_done, 8);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_done, 8);
+    mbar_init(acc_full, 1);
+    mbar_init(drained, 1);
+    for (int i = 0; i < kMaskRing; ++i) {
+      mbar_init(m_full(i), 1);
+      mbar_init(m_empty(i), 8);
+    }
+    s_bail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (KV && tile_rows < 128) {
+    // rows that no load writes take part in the sums over rows: zeros instead of what the memory held
+    for (int s = 0; s < kStages * NSUB; ++s)
+      for (int i = threadIdx.x; i < (128 - tile_rows) * 8; i += kAttThreads)
+        smem_zero16(s_ring + s * kTileBytes + tile_rows * 128 + i * 16);
+    fence_async_smem();
+  }
+  if (warp == 9) tmem_alloc<512>(&s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const Bail bail{&s_bail, a.p.status};
+  const uint32_t x_bytes = KV ? kStageBytes : (uint32_t)(NSUB * tile_rows * 128);
+  const uint32_t y_bytes = KV ? (uint32_t)(NSUB * tile_rows * 128) : kStageBytes;
+  // dQ: keys that may not be attended are cleared before they meet dS
+  const auto needs_fix = [&](int t) { return !KV && (masked || ((t0 + t + 1) * 128 > keys && keys < a.p.Lk)); };
+  grid_dependency_wait();  // delta comes from the kernel before
+
+  if (warp >= 8) {
+    set_registers_down<80>();
+    if (warp == 8 && n > 0) {
+      // ---- loads -------------------------------------------------------------------------------------------------
+      const int qb = a.p.q_shared ? 0 : b;
+      const auto load_rows = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int tile, int batch) {
+        for (int x = 0; x < NSUB; ++x) tma_load_5d(dst + x * kTileBytes, map, bar, 64 * x, 0, g, tile * pl.TL, batch);
+      };
+      const auto load_keys = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int tile) {
+        for (int x = 0; x < NSUB; ++x) tma_load_4d(dst + x * kTileBytes, map, bar, 64 * x, g, tile * 128, b);
+      };
+      const bool leader = elect_one();
+      if (leader) {
+        mbar_expect(x_full, 2 * x_bytes);
+        if (KV) {
+          load_keys(s_x, &a.x0, x_full, xt);
+          load_keys(s_x + kStageBytes, &a.x1, x_full, xt);
+        } else {
+          load_rows(s_x, &a.x0, x_full, xt, qb);
+          load_rows(s_x + kStageBytes, &a.x1, x_full, xt, b);
+        }
+      }
+      int slot = 0;
+      bool ok = true;
+      const auto load = [&](const CUtensorMap* map, int t, int batch) {
+        const int s = slot % kStages;
+        if (ok && slot >= kStages) ok = warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
+        if (!ok) return;
+        if (leader) {
+          mbar_expect(full(s), y_bytes);
+          if (KV)
+            load_rows(s_ring + s * kStageBytes, map, full(s), t0 + t, batch);
+          else
+            load_keys(s_ring + s * kStageBytes, map, full(s), t0 + t);
+        }
+        __syncwarp();
+        ++slot;
+      };
+      for (int t = 0; t < n && ok; ++t) {
+        load(&a.y0, t, qb);
+        load(&a.y1, t, b);
+      }
+      if (!ok) {
+        // nothing may be left in flight when the block ends
+        mbar_drain(x_full, 0);
+        for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) mbar_drain(full(i % kStages), (i / kStages) & 1);
+      }
+    } else if (warp == 9 && n > 0) {
+      const bool leader = elect_one();
+      // ---- matrix instructions -----------------------------------------------------------------------------------
+      const int ksteps = (a.p.D + 15) / 16;
+      const uint32_t i_s = umma_instr<T>(128, false, a.p.scale < 0.0f), i_dp = umma_instr<T>(128, false, false),
+                     i_acc = umma_instr<T>(ksteps * 16, true, false);
+      uint32_t fix_parity = 0;
+      bool ok = warp_wait(x_full, 0, bail);
+      const auto commit = [&](uint32_t bar) {
+        if (leader) umma_commit(bar);
+        __syncwarp();
+      };
+      const auto stage = [&](int slot) { return s_ring + (slot % kStages) * kStageBytes; };
+      const auto wait_full = [&](int slot) { ok = ok && warp_wait(full(slot % kStages), (slot / kStages) & 1, bail); };
+      const auto product = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t instr) {  // X Y^T over the head's width
+        if (leader) {
+#pragma unroll
+          for (int i = 0; i < NSUB; ++i) {
+            const uint64_t da = desc_k_major(x + i * kTileBytes), db = desc_k_major(y + i * kTileBytes);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (i * 4 + k < ksteps) umma_ss(d, da + 2 * k, db + 2 * k, instr, i + k > 0);
+          }
+        }
+        __syncwarp();
+      };
+      const auto accumulate = [&](uint32_t d, uint32_t t, uint32_t y, bool first) {  // 16-bit tile in tensor memory times Y
+        if (leader) {
+          const uint64_t db = desc_mn_major(y);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) umma_ts(d, t + (k < 4 ? 8 * k : 32 + 8 * k), db + 128 * k, i_acc, !first || k > 0);
+        }
+        __syncwarp();
+      };
+      const auto scores = [&](int t) {
+        wait_full(2 * t);
+        if (needs_fix(t)) {
+          const int s = (2 * t) % kStages;
+          ok = ok && warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
+          fix_parity ^= 1u << s;
+        }
+        if (!ok) return;
+        tc_fence_after();
+        product(tmem, s_x, stage(2 * t), i_s);
+        commit(s_full);
+      };
+      const auto dprobs = [&](int t) {
+        wait_full(2 * t + 1);
+        if (!ok) return;
+        tc_fence_after();
+        product(tmem + 128, s_x + kStageBytes, stage(2 * t + 1), i_dp);
+        commit(dp_full);
+        if (!KV) commit(empty((2 * t + 1) % kStages));
+      };
+      scores(0);
+      if (ok) dprobs(0);
+      for (int t = 0; t < n && ok; ++t) {
+        ok = warp_wait(p_done, t & 1, bail);
+        if (!ok) break;
+        if (KV) {
+          tc_fence_after();
+          accumulate(tmem + 384, tmem, stage(2 * t + 1), t == 0);
+          commit(empty((2 * t + 1) % kStages));
+        }
+        if (t + 1 < n) scores(t + 1);
+        ok = ok && warp_wait(ds_done, t & 1, bail);
+        if (!ok) break;
+        tc_fence_after();
+        accumulate(tmem + 256, tmem + 128, stage(2 * t), t == 0);
+        commit(empty((2 * t) % kStages));
+        if (t + 1 < n) dprobs(t + 1);
+      }
+      commit(ok ? acc_full : drained);
+      if (!ok) mbar_drain(drained, 0);
+    } else if (!KV && warp == 10 && n > 0 && (masked || keys < a.p.Lk)) {
+      bool ok = true;
+      // ---- key mask, keys that may not be attended -----------------------------------------------------------------
+      const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
+      for (int t = 0; t < n && ok; ++t) {
+        if (!needs_fix(t)) continue;
+        const int s = (2 * t) % kStages;
+        uint32_t word[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = (t0 + t) * 128 + 32 * i + lane;
+          word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
+        }
+        if (masked) {
+          const int m = t % kMaskRing;
+          if (t >= kMaskRing) ok = warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
+          if (!ok) break;
+          if (lane < 4) s_mask[m][lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m_full(m));
+        }
+        ok = warp_wait(full(s), ((2 * t) / kStages) & 1, bail);
+        if (!ok) break;
+        if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
+          for (int r = lane >> 3; r < 128; r += 4) {
+            const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
+            if ((w >> (r & 31)) & 1) continue;
+            for (int x = 0; x < NSUB; ++x)
+              smem_zero16(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16);
+          }
+          fence_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(fixed(s));
+      }
+    }
+  } else {
+    // ---- P and dS ----------------------------------------------------------------------------------------------------
+    set_registers_up<208>();
+    const int h = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_s = lanes + 64 * h, t_dp = lanes + 128 + 64 * h;
+    const long long row = (long long)xt * tile_rows + r;             // dQ
+    const bool row_live = !KV && r < tile_rows && row < rows;
+    const int key = xt * 128 + r;                                    // dK, dV
+    const float* nlse = a.nlse + ((long long)bg * pl.row_tiles + (KV ? t0 : xt)) * 128;
+    const float* ndelta = a.ndelta + ((long long)bg * pl.row_tiles + (KV ? t0 : xt)) * 128;
+    const float nl = KV ? 0.0f : nlse[r], nd = KV ? 0.0f : ndelta[r];
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      const int mr = t % kMaskRing;
+      uint32_t word[2] = {kFull, kFull};
+      if (!KV && masked) {
+        ok = warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
+        if (!ok) break;
+        word[0] = s_mask[mr][2 * h];
+        word[1] = s_mask[mr][2 * h + 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m_empty(mr));
+      } else if (!KV && (t0 + t + 1) * 128 > keys) {
+        const int have = keys - (t0 + t) * 128 - 64 * h;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
+      }
+      const bool cut = (word[0] & word[1]) != kFull;
+      ok = warp_wait(s_full, t & 1, bail);
+      if (!ok) break;
+      tc_fence_after();
+      float p[64];
+      tmem_ld32(t_s, p);
+      tmem_ld32(t_s + 32, p + 32);
+      tmem_wait_ld();
+      if (!KV) {  // S may be overwritten
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_done);
+      }
+#pragma unroll
+      for (int x = 0; x < 64; x += 4) {
+        float4 l = make_float4(nl, nl, nl, nl);
+        if (KV) l = *reinterpret_cast<const float4*>(nlse + 128 * t + 64 * h + x);
+        const float2 e0 = fma2(make_float2(p[x], p[x + 1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
+        const float2 e1 = fma2(make_float2(p[x + 2], p[x + 3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
+        p[x] = exp2_fast(e0.x);
+        p[x + 1] = exp2_fast(e0.y);
+        p[x + 2] = exp2_fast(e1.x);
+        p[x + 3] = exp2_fast(e1.y);
+      }
+      if (KV) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) packed[x] = pack2<T>(p[2 * x], p[2 * x + 1]);
+        tmem_st32(t_s, packed);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_done);
+      }
+      ok = warp_wait(dp_full, t & 1, bail);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t packed[32];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float dp[32];
+        tmem_ld32(t_dp + 32 * y, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          float4 d = make_float4(nd, nd, nd, nd);
+          if (KV) d = *reinterpret_cast<const float4*>(ndelta + 128 * t + 64 * h + 32 * y + x);
+          const float* q = p + 32 * y + x;
+          float2 s0 = add2(make_float2(dp[x], dp[x + 1]), make_float2(d.x, d.y));
+          float2 s1 = add2(make_float2(dp[x + 2], dp[x + 3]), make_float2(d.z, d.w));
+          s0 = make_float2(s0.x * q[0], s0.y * q[1]);
+          s1 = make_float2(s1.x * q[2], s1.y * q[3]);
+          if (cut) {  // a select, not a product: what stands there may be NaN
+            if (!((word[y] >> x) & 1)) s0.x = 0.0f;
+            if (!((word[y] >> (x + 1)) & 1)) s0.y = 0.0f;
+            if (!((word[y] >> (x + 2)) & 1)) s1.x = 0.0f;
+            if (!((word[y] >> (x + 3)) & 1)) s1.y = 0.0f;
+          }
+          packed[16 * y + x / 2] = pack2<T>(s0.x, s0.y);
+          packed[16 * y + x / 2 + 1] = pack2<T>(s1.x, s1.y);
+        }
+      }
+      tmem_st32(t_dp, packed);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_done);
+    }
+    if (ok && n > 0) ok = warp_wait(acc_full, 0, bail);
+    tc_fence_after();
+    // ---- output: dQ column chunks in turn, or dK by the first group and dV by the second --------------------------------
+    const int d16 = (a.p.D + 15) / 16 * 16;
+    const bool parted = pl.splits > 1;
+    const bool live = KV ? key < a.p.Lk : row_live;
+    bool zero = n == 0;
+    if (KV && live) zero = zero || key >= keys || !att_allowed(a.p, b, key);
+    const long long l = KV ? 0 : row / pl.G;
+    const long long at = KV ? (((long long)b * a.p.Lk + key) * a.p.Hkv + g) * a.p.D
+                            : (((long long)b * a.p.Lq + l) * a.p.Hq + g * pl.G + (row - l * pl.G)) * a.p.D;
+    const long long whole = KV ? (long long)a.p.B * a.p.Lk * a.p.Hkv * a.p.D : (long long)a.p.B * a.p.Lq * a.p.Hq * a.p.D;
+    T* dst = reinterpret_cast<T*>(KV && h ? a.g1 : a.g0) + at;
+    float* dpart = (KV && h ? a.part1 : a.part0) + split * whole + at;
+    const float f = KV && h ? 1.0f : a.p.scale;
+    __syncwarp();
+#pragma unroll 1
+    for (int x = KV ? 0 : 32 * h; x < d16; x += KV ? 32 : 64) {
+      float o[32];
+      if (n > 0) {
+        tmem_ld32(lanes + (KV && h ? 384 : 256) + x, o);
+        tmem_wait_ld();
+      }
+      if (zero) {
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+      }
+      if (live) {
+        if (parted)
+          store_row32(dpart + x, o, 1.0f, a.p.D - x);
+        else
+          store_row16<T>(dst + x, o, f, a.p.D - x);
+      }
+      __syncwarp();
+    }
+    tc_fence_before();
+  }
+  grid_dependency_trigger();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_free<512>(tmem);
+  }
+}
+
+// g[i] = f * (sum of the parts in order); four elements a thread
+template <typename T>
+__global__ void __launch_bounds__(256) att_sum_kernel(const float* __restrict__ part, int splits, long long count, float f, T* __restrict__ g) {
+  grid_dependency_wait();
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (long long)gridDim.x * 1024) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(part + k * count + i);
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    uint2 w;
+    w.x = pack2<T>(s.x * f, s.y * f);
+    w.y = pack2<T>(s.z * f, s.w * f);
+    *reinterpret_cast<uint2*>(g + i) = w;
+  }
+}
+
+// -lse and -delta = -<out, grad_out> of every row of the padded row tiles: eight lanes a row, 16 bytes a load
+template <typename T>
+__global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ FbevAttention p, int TL, int row_tiles, const T* __restrict__ out,
+                                                       const T* __restrict__ go, const float* __restrict__ lse, float* __restrict__ nlse,
+                                                       float* __restrict__ ndelta) {
+  const long long rows = att_rows(p), at = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int lane = threadIdx.x & 7, G = p.Hq / p.Hkv;
+  const long long tile = at >> 7, bg = tile / row_tiles;
+  const int r = (int)(at & 127);
+  const long long row = (tile - bg * row_tiles) * TL * G + r;
+  const bool there = bg < (long long)p.B * p.Hkv, live = there && r < TL * G && row < rows;
+  float d = 0.0f;
+  if (live) {
+    const long long b = bg / p.Hkv, g = bg - b * p.Hkv, l = row / G;
+    const long long head = ((b * p.Lq + l) * p.Hq + g * G + (row - l * G)) * p.D;
+    for (int c = lane * 8; c < p.D; c += 64) {
+      const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(out + head + c);
+      const Pack<T, 8> y = *reinterpret_cast<const Pack<T, 8>*>(go + head + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d = fmaf(to_float(x.v[e]), to_float(y.v[e]), d);
+    }
+  }
+#pragma unroll
+  for (int s = 4; s > 0; s >>= 1) d += __shfl_xor_sync(kFull, d, s);
+  if (there && lane == 0) {
+    nlse[at] = live ? -lse[bg * att_rows_padded(p) + row] : -INFINITY;
+    ndelta[at] = -d;
+  }
+  grid_dependency_trigger();
+}
+
+}  // namespace fbev

@@ -157,24 +157,27 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
 
   if (warp >= 8) {
     set_registers_down<80>();
-    if (warp == 8 && lane == 0 && n > 0) {
+    if (warp == 8 && n > 0) {
       // ---- loads -------------------------------------------------------------------------------------------------
-      tma_prefetch(&a.q);
-      tma_prefetch(&a.k);
-      tma_prefetch(&a.v);
-      mbar_expect(q_full, (uint32_t)(tiles * NSUB * tile_rows * 128));
-      for (int i = 0; i < tiles; ++i)
-        for (int x = 0; x < NSUB; ++x)
-          tma_load_5d(s_q + i * kStageBytes + x * kTileBytes, &a.q, q_full, 64 * x, 0, g, (2 * rb + i) * pl.TL, a.p.q_shared ? 0 : b);
+      const bool leader = elect_one();
+      if (leader) {
+        mbar_expect(q_full, (uint32_t)(tiles * NSUB * tile_rows * 128));
+        for (int i = 0; i < tiles; ++i)
+          for (int x = 0; x < NSUB; ++x)
+            tma_load_5d(s_q + i * kStageBytes + x * kTileBytes, &a.q, q_full, 64 * x, 0, g, (2 * rb + i) * pl.TL, a.p.q_shared ? 0 : b);
+      }
       int slot = 0;
       bool ok = true;
       const auto load = [&](const CUtensorMap* map, int t) {
         const int s = slot % kStages;
-        if (ok && slot >= kStages) ok = mbar_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
+        if (ok && slot >= kStages) ok = warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
         if (!ok) return;
-        mbar_expect(full(s), kStageBytes);
-        for (int x = 0; x < NSUB; ++x)
-          tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, (t0 + t) * 128, b);
+        if (leader) {
+          mbar_expect(full(s), kStageBytes);
+          for (int x = 0; x < NSUB; ++x)
+            tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, (t0 + t) * 128, b);
+        }
+        __syncwarp();
         ++slot;
       };
       load(&a.k, 0);
@@ -186,48 +189,54 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       }
       if (!ok) {
         // nothing may be left in flight when the block ends
-        mbar_wait(q_full, 0, bail);
-        for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) {
-          const long long begin = clock64();
-          while (!mbar_try(full(i % kStages), (i / kStages) & 1) && clock64() - begin < 1000000000ll) {
-          }
-        }
+        mbar_drain(q_full, 0);
+        for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) mbar_drain(full(i % kStages), (i / kStages) & 1);
       }
-    } else if (warp == 9 && lane == 0 && n > 0) {
+    } else if (warp == 9 && n > 0) {
+      const bool leader = elect_one();
       // ---- matrix instructions -----------------------------------------------------------------------------------
       const bool negative = a.p.scale < 0.0f;
       const int ksteps = (a.p.D + 15) / 16;
       const uint32_t i_s = umma_instr<T>(128, false, negative), i_o = umma_instr<T>(ksteps * 16, true, false);
       uint32_t fix_parity = 0;
       int slot = 0;
-      bool ok = mbar_wait(q_full, 0, bail);
+      bool ok = warp_wait(q_full, 0, bail);
       const auto take = [&]() {  // next tile of the ring, as shared-memory address
         const int s = slot % kStages;
-        ok = ok && mbar_wait(full(s), (slot / kStages) & 1, bail);
+        ok = ok && warp_wait(full(s), (slot / kStages) & 1, bail);
         ++slot;
         return s;
       };
+      const auto commit = [&](uint32_t bar) {
+        if (leader) umma_commit(bar);
+        __syncwarp();
+      };
       const auto scores = [&](int i, int s) {
         tc_fence_after();
+        if (leader) {
 #pragma unroll
-        for (int x = 0; x < NSUB; ++x) {
-          const uint64_t da = desc_k_major(s_q + (pair ? 0 : i) * kStageBytes + x * kTileBytes);
-          const uint64_t db = desc_k_major(s_ring + s * kStageBytes + x * kTileBytes);
+          for (int x = 0; x < NSUB; ++x) {
+            const uint64_t da = desc_k_major(s_q + (pair ? 0 : i) * kStageBytes + x * kTileBytes);
+            const uint64_t db = desc_k_major(s_ring + s * kStageBytes + x * kTileBytes);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (x * 4 + k < ksteps) umma_ss(tmem + 128 * i, da + 2 * k, db + 2 * k, i_s, x + k > 0);
+            for (int k = 0; k < 4; ++k)
+              if (x * 4 + k < ksteps) umma_ss(tmem + 128 * i, da + 2 * k, db + 2 * k, i_s, x + k > 0);
+          }
         }
-        umma_commit(s_full(i));
+        commit(s_full(i));
       };
       const auto values = [&](int i, int s, bool first) {
         tc_fence_after();
-        const uint64_t db = desc_mn_major(s_ring + s * kStageBytes);
+        if (leader) {
+          const uint64_t db = desc_mn_major(s_ring + s * kStageBytes);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) umma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, db + 128 * k, i_o, !first || k > 0);
+          for (int k = 0; k < 8; ++k) umma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, db + 128 * k, i_o, !first || k > 0);
+        }
+        __syncwarp();
       };
       const auto fix_wait = [&](int t, int s) {
         if (!needs_fix(t)) return;
-        ok = ok && mbar_wait(fixed(s), (fix_parity >> s) & 1, bail);
+        ok = ok && warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
         fix_parity ^= 1u << s;
       };
       if (pair) {
@@ -235,54 +244,52 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           const int s = take();
           if (!ok) break;
           scores(t, s);
-          umma_commit(empty(s));
+          commit(empty(s));
         }
         for (int t = 0; t < n && ok; ++t) {
           const int i = t & 1, s = take();
           fix_wait(t, s);
-          ok = ok && mbar_wait(p_full(i), (t >> 1) & 1, bail);
+          ok = ok && warp_wait(p_full(i), (t >> 1) & 1, bail);
           if (!ok) break;
           values(i, s, t < 2);
-          umma_commit(empty(s));
-          if (t + 2 >= n) umma_commit(o_full(i));
+          commit(empty(s));
+          if (t + 2 >= n) commit(o_full(i));
           if (t + 2 < n) {
             const int sk = take();
             if (!ok) break;
             scores(i, sk);
-            umma_commit(empty(sk));
+            commit(empty(sk));
           }
         }
       } else {
         const int sk0 = take();
         if (ok) {
           for (int i = 0; i < tiles; ++i) scores(i, sk0);
-          umma_commit(empty(sk0));
+          commit(empty(sk0));
         }
         for (int t = 0; t < n && ok; ++t) {
           const int s = take();
           fix_wait(t, s);
           int sk = 0;
           for (int i = 0; i < tiles; ++i) {
-            ok = ok && mbar_wait(p_full(i), t & 1, bail);
+            ok = ok && warp_wait(p_full(i), t & 1, bail);
             if (!ok) break;
             values(i, s, t == 0);
-            if (i == tiles - 1) umma_commit(empty(s));
+            if (i == tiles - 1) commit(empty(s));
             if (t + 1 == n) {
-              umma_commit(o_full(i));
+              commit(o_full(i));
               continue;
             }
             if (i == 0) sk = take();
             if (!ok) break;
             scores(i, sk);
-            if (i == tiles - 1) umma_commit(empty(sk));
+            if (i == tiles - 1) commit(empty(sk));
           }
         }
       }
       if (!ok) {
-        umma_commit(drained);
-        const long long begin = clock64();
-        while (!mbar_try(drained, 0) && clock64() - begin < 1000000000ll) {
-        }
+        commit(drained);
+        mbar_drain(drained, 0);
       }
     } else if (warp == 10 && n > 0 && (masked || keys < a.p.Lk)) {
       // ---- key mask, values that may not be attended ---------------------------------------------------------------
@@ -302,14 +309,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         }
         if (masked) {
           const int m = t % kMaskRing;
-          if (t >= kMaskRing) ok = mbar_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
-          ok = __all_sync(kFull, ok);
+          if (t >= kMaskRing) ok = warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
           if (!ok) break;
           if (lane < 4) s_mask[m][lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
           __syncwarp();
           if (lane == 0) mbar_arrive(m_full(m));
         }
-        ok = __all_sync(kFull, mbar_wait(full(s), round & 1, bail));
+        ok = warp_wait(full(s), round & 1, bail);
         if (!ok) break;
         if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
           // a row's 128 bytes: eight lanes, four rows at a time (the swizzle permutes within the row, zeros do not care)
@@ -317,9 +323,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
             const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
             if ((w >> (r & 31)) & 1) continue;
             for (int x = 0; x < NSUB; ++x)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16),
-                           "r"(0u)
-                           : "memory");
+              smem_zero16(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16);
           }
           fence_async_smem();
         }
@@ -349,7 +353,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         bool cut = false;
         if (masked) {
           const int mr = t % kMaskRing;
-          ok = __all_sync(kFull, mbar_wait(m_full(mr), (t / kMaskRing) & 1, bail));
+          ok = warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
           if (!ok) break;
 #pragma unroll
           for (int x = 0; x < 4; ++x) word[x] = s_mask[mr][x];
@@ -362,7 +366,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           for (int x = 0; x < 4; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
           cut = true;
         }
-        ok = __all_sync(kFull, mbar_wait(s_full(i), j & 1, bail));
+        ok = warp_wait(s_full(i), j & 1, bail);
         if (!ok) break;
         tc_fence_after();
         float s[128];
@@ -392,7 +396,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
               tmem_wait_ld();
 #pragma unroll
               for (int y = 0; y < 32; ++y) o[y] *= back;
-              tmem_st32(t_o + x, reinterpret_cast<const uint32_t*>(o));
+              tmem_st32(t_o + x, o);
             }
           }
         }
@@ -415,9 +419,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(i));
       }
-      if (ok && mine > 0) ok = __all_sync(kFull, mbar_wait(o_full(i), 0, bail));
+      if (ok && mine > 0) ok = warp_wait(o_full(i), 0, bail);
       // the second group is about to write over the ring: the first group's tiles must have been consumed too
-      if (ok && pair && i == 1 && mine > 0) ok = __all_sync(kFull, mbar_wait(o_full(0), 0, bail));
+      if (ok && pair && i == 1 && mine > 0) ok = warp_wait(o_full(0), 0, bail);
+      __syncwarp();
       tc_fence_after();
     }
     // ---- output ------------------------------------------------------------------------------------------------------
@@ -456,7 +461,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       const long long at = (long long)split * a.p.B * a.p.Hkv + bg;
       float* dpart = a.part + (at * rows + row) * a.p.D;
       const float* s_join = reinterpret_cast<const float*>(s_raw + (s_ring - smem_addr(s_raw)));
-      if (works || n == 0) {
+      __syncwarp();
+      if (works) {
 #pragma unroll 1
         for (int x = 0; x < d16; x += 32) {
           float o[32];
@@ -471,11 +477,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = o[y] * f0 + s_join[(x + y) * 128 + r] * f1;
           }
-          if (!live) continue;
-          if (parted)
-            store_row32(dpart + x, o, inv, a.p.D - x);
-          else
-            store_row16<T>(dst + x, o, inv, a.p.D - x);
+          if (live) {
+            if (parted)
+              store_row32(dpart + x, o, inv, a.p.D - x);
+            else
+              store_row16<T>(dst + x, o, inv, a.p.D - x);
+          }
+          __syncwarp();
         }
       }
       if (live) {

@@ -11,6 +11,7 @@
 #include "fbev_query.h"
 #include "fbev_attention.cuh"
 #include "fbev_attention_tc.cuh"
+#include "fbev_attention_grad_tc.cuh"
 #include "fbev_norm.cuh"
 #include "fbev_rotary.cuh"
 
@@ -214,9 +215,95 @@ static int attention_forward(const FbevAttention& p, T* out, float* lse, cudaStr
   return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
 }
 
+// blocks along the other side when this side's tiles leave SMs idle
+static AttGradPlan gradient_plan(const FbevAttention& p, bool kv) {
+  AttGradPlan pl{};
+  pl.G = p.Hq / p.Hkv;
+  pl.TL = 128 / pl.G;
+  pl.row_tiles = (p.Lq + pl.TL - 1) / pl.TL;
+  pl.key_tiles = (p.Lk + 127) / 128;
+  const long long blocks = (long long)p.B * p.Hkv * (kv ? pl.key_tiles : pl.row_tiles);
+  const int other = kv ? pl.row_tiles : pl.key_tiles;
+  long long splits = blocks < kSms ? kSms / blocks : 1;
+  if (splits > other) splits = other;
+  pl.per_split = (int)((other + splits - 1) / splits);
+  pl.splits = (other + pl.per_split - 1) / pl.per_split;
+  return pl;
+}
+static size_t gradient_part_bytes(const FbevAttention& p, bool kv) {  // of one of the gradients
+  const AttGradPlan pl = gradient_plan(p, kv);
+  if (pl.splits == 1) return 0;
+  return round_up((size_t)pl.splits * p.B * (kv ? (size_t)p.Lk * p.Hkv : (size_t)p.Lq * p.Hq) * p.D * 4, 256);
+}
+static size_t delta_bytes(const FbevAttention& p) { return round_up((size_t)p.B * p.Hkv * att_rows_padded(p) * 4, 256); }
+static size_t stat_bytes(const FbevAttention& p) {  // -lse or -delta by row tile
+  return (size_t)p.B * p.Hkv * gradient_plan(p, false).row_tiles * 512;
+}
+// both statistics, then the parts of dQ, and after those are summed the parts of dK and dV in the same place; room for the
+// delta of the row kernels too, which take over when an address of the gradients is not aligned
+static size_t backward_workspace(const FbevAttention& p) {
+  if (!on_tensor_cores(p)) return delta_bytes(p);
+  const size_t q = gradient_part_bytes(p, false), kv = 2 * gradient_part_bytes(p, true);
+  return delta_bytes(p) + 2 * stat_bytes(p) + (q > kv ? q : kv);
+}
+
+template <typename T, int NSUB, bool KV>
+static int tensor_gradient(const FbevAttention& p, const T* go, T* g0, T* g1, cudaStream_t st) {
+  static std::atomic<uint64_t> granted{0};
+  AttGradArgs a;
+  a.p = p;
+  a.pl = gradient_plan(p, KV);
+  AttPlan rows{};
+  rows.G = a.pl.G;
+  rows.TL = a.pl.TL;
+  const int64_t go_stride[3] = {(int64_t)p.Lq * p.Hq * p.D, (int64_t)p.Hq * p.D, p.D};
+  int rc = allow_smem(att_grad_kernel<T, NSUB, KV>, AttGradShape<NSUB>::kSmem, granted);
+  if (rc == FBEV_OK) rc = encode_rows(KV ? &a.y0 : &a.x0, p, rows, p.q, p.q_stride, p.q_shared != 0);
+  if (rc == FBEV_OK) rc = encode_rows(KV ? &a.y1 : &a.x1, p, rows, go, go_stride, false);
+  if (rc == FBEV_OK) rc = encode_keys(KV ? &a.x0 : &a.y0, p, p.k, p.k_stride);
+  if (rc == FBEV_OK) rc = encode_keys(KV ? &a.x1 : &a.y1, p, p.v, p.v_stride);
+  if (rc != FBEV_OK) return rc;
+  char* ws = reinterpret_cast<char*>(p.workspace);
+  a.nlse = reinterpret_cast<const float*>(ws);
+  a.ndelta = reinterpret_cast<const float*>(ws + stat_bytes(p));
+  a.part0 = reinterpret_cast<float*>(ws + 2 * stat_bytes(p));
+  a.part1 = reinterpret_cast<float*>(ws + 2 * stat_bytes(p) + gradient_part_bytes(p, KV));
+  a.g0 = g0;
+  a.g1 = g1;
+  a.c = score_factor(p);
+  const long long blocks = (long long)p.B * p.Hkv * (KV ? a.pl.key_tiles : a.pl.row_tiles) * a.pl.splits;
+  launch_next(att_grad_kernel<T, NSUB, KV>, (unsigned)blocks, kAttThreads, AttGradShape<NSUB>::kSmem, st, a);
+  if (a.pl.splits > 1) {
+    const long long count = (long long)p.B * (KV ? (long long)p.Lk * p.Hkv : (long long)p.Lq * p.Hq) * p.D;
+    const long long want = (count / 4 + 255) / 256;
+    const unsigned grid = (unsigned)(want < kSms * 8 ? want : kSms * 8);
+    launch_next(att_sum_kernel<T>, grid, 256, 0, st, (const float*)a.part0, a.pl.splits, count, p.scale, g0);
+    if (KV) launch_next(att_sum_kernel<T>, grid, 256, 0, st, (const float*)a.part1, a.pl.splits, count, 1.0f, g1);
+  }
+  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+
+template <typename T, int NSUB>
+static int tensor_backward(const FbevAttention& p, const T* out, const float* lse, const T* go, T* gq, T* gk, T* gv, cudaStream_t st) {
+  const AttGradPlan pl = gradient_plan(p, false);
+  float* nlse = reinterpret_cast<float*>(p.workspace);
+  float* ndelta = reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + stat_bytes(p));
+  const unsigned blocks = (unsigned)((long long)p.B * p.Hkv * pl.row_tiles * 4);
+  att_stat_kernel<T><<<blocks, 256, 0, st>>>(p, pl.TL, pl.row_tiles, out, go, lse, nlse, ndelta);
+  int rc = cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+  if (rc == FBEV_OK && gq) rc = tensor_gradient<T, NSUB, false>(p, go, gq, (T*)nullptr, st);
+  if (rc == FBEV_OK && gk) rc = tensor_gradient<T, NSUB, true>(p, go, gk, gv, st);
+  return rc;
+}
+
 template <typename T>
 static int attention_backward(const FbevAttention& p, const T* out, const float* lse, const T* go, T* gq, T* gk, T* gv,
                               cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    const uintptr_t all = (uintptr_t)out | (uintptr_t)go | (uintptr_t)gq | (uintptr_t)gk | (uintptr_t)gv;
+    if (on_tensor_cores(p) && all % 16 == 0)
+      return p.D <= 64 ? tensor_backward<T, 1>(p, out, lse, go, gq, gk, gv, st) : tensor_backward<T, 2>(p, out, lse, go, gq, gk, gv, st);
+  }
   float* delta = reinterpret_cast<float*>(p.workspace);
   const long long units = att_rows(p) * p.B * p.Hkv, keys = (long long)p.B * p.Lk * p.Hkv;
   if (units > 0) att_delta_kernel<T><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(p, out, go, delta);
@@ -238,7 +325,7 @@ size_t fbev_cross_attention_lse_count(const FbevAttention* p) {
 
 size_t fbev_cross_attention_workspace_bytes(const FbevAttention* p, int backward) {
   if (check_attention(p) != FBEV_OK) return 0;
-  return backward ? round_up(fbev_cross_attention_lse_count(p) * 4, 256) : forward_workspace(*p);
+  return backward ? backward_workspace(*p) : forward_workspace(*p);
 }
 
 static int check_workspace(const FbevAttention* p, int backward) {

@@ -58,6 +58,26 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const B
   }
 }
 
+// the same for a whole warp, which stays together
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
+  return __all_sync(kFull, mbar_wait(bar, parity, bail));
+}
+// for a while only, whatever became of the others: before a block ends early
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity) && clock64() - t0 < 1000000000ll) {
+  }
+}
+
+// One lane of a converged warp, the same each time.  Loads and matrix instructions are issued by it from loops that the
+// whole warp runs: their descriptors live in uniform registers, which a loop run by one lane alone would share with lanes
+// that are elsewhere.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(pred));
+  return pred != 0;
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
@@ -73,6 +93,10 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+__device__ __forceinline__ void smem_zero16(uint32_t addr) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
 }
 
 // order generic stores to shared memory before later reads by TMA or the tensor cores
@@ -92,16 +116,16 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of this thread's lane (the warp's 32 lanes start at lane 32 * (warp % 4), which the address carries)
+// 32 columns of this thread's lane (the warp's 32 lanes start at lane 32 * (warp % 4), which the address carries).  The whole
+// warp takes part: where lanes went separate ways before, a __syncwarp or a vote comes first.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
       "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-        "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
-        "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
-        "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+        "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]),
+        "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]),
+        "=f"(r[30]), "=f"(r[31])
       : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
@@ -113,6 +137,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
       "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]),
       "r"(u[31])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float* r) {
+  uint32_t u[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(r[i]);
+  tmem_st32(addr, u);
 }
 
 // ---- matrix instructions --------------------------------------------------------------------------------------------
