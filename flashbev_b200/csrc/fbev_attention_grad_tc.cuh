@@ -89,10 +89,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   const auto m_full = [&](int i) { return drained + 8 + 8 * i; };
   const auto m_empty = [&](int i) { return drained + 8 + 8 * (kMaskRing + i); };
 
+  // dQ: keys that may not be attended are cleared before they meet dS, by a warp that follows the ring (as in the forward)
+  const bool fixes = !KV && (masked || keys < a.p.Lk);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), fixes ? 2 : 1);
       mbar_init(fixed(s), 1);
     }
     mbar_init(x_full, 1);
@@ -124,8 +126,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   const Bail bail{&s_bail, a.p.status};
   const uint32_t x_bytes = KV ? kStageBytes : (uint32_t)(NSUB * tile_rows * 128);
   const uint32_t y_bytes = KV ? (uint32_t)(NSUB * tile_rows * 128) : kStageBytes;
-  // dQ: keys that may not be attended are cleared before they meet dS
-  const auto needs_fix = [&](int t) { return !KV && (masked || ((t0 + t + 1) * 128 > keys && keys < a.p.Lk)); };
+  const auto needs_fix = [&](int t) { return fixes && (masked || (t0 + t + 1) * 128 > keys); };
   grid_dependency_wait();  // delta comes from the kernel before
 
   if (warp >= 8) {
@@ -249,18 +250,23 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       }
       commit(ok ? acc_full : drained);
       if (!ok) mbar_drain(drained, 0);
-    } else if (!KV && warp == 10 && n > 0 && (masked || keys < a.p.Lk)) {
-      bool ok = true;
+    } else if (fixes && warp == 10 && n > 0) {
       // ---- key mask, keys that may not be attended -----------------------------------------------------------------
       const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
+      bool ok = true;
+      const auto release = [&](int s) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
+      };
       for (int t = 0; t < n && ok; ++t) {
-        if (!needs_fix(t)) continue;
-        const int s = (2 * t) % kStages;
-        uint32_t word[4];
+        uint32_t word[4] = {kFull, kFull, kFull, kFull};
+        const bool fix = needs_fix(t);
+        if (fix) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = (t0 + t) * 128 + 32 * i + lane;
-          word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
+          for (int i = 0; i < 4; ++i) {
+            const int j = (t0 + t) * 128 + 32 * i + lane;
+            word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
+          }
         }
         if (masked) {
           const int m = t % kMaskRing;
@@ -270,19 +276,25 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive(m_full(m));
         }
+        const int s = (2 * t) % kStages, s1 = (2 * t + 1) % kStages;
         ok = warp_wait(full(s), ((2 * t) / kStages) & 1, bail);
         if (!ok) break;
-        if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
-          for (int r = lane >> 3; r < 128; r += 4) {
-            const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
-            if ((w >> (r & 31)) & 1) continue;
-            for (int x = 0; x < NSUB; ++x)
-              smem_zero16(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16);
+        if (fix) {
+          if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
+            for (int r = lane >> 3; r < 128; r += 4) {
+              const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
+              if ((w >> (r & 31)) & 1) continue;
+              for (int x = 0; x < NSUB; ++x) smem_zero16(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16);
+            }
+            fence_async_smem();
           }
-          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(fixed(s));
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(fixed(s));
+        release(s);
+        ok = warp_wait(full(s1), ((2 * t + 1) / kStages) & 1, bail);
+        if (!ok) break;
+        release(s1);
       }
     }
   } else {

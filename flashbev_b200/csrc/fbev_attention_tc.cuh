@@ -126,10 +126,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   const int live_rows = pair ? (int)(left < tile_rows ? left : tile_rows) : 128;
   const int live_warps = (live_rows + 31) / 32;
 
+  // The warp that clears values follows the ring tile by tile and has to let go of each stage too: a barrier tells only
+  // the last phase from the one before, so no one may fall a round behind.
+  const bool fixes = masked || keys < a.p.Lk;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), fixes ? 2 : 1);
       mbar_init(fixed(s), 1);
     }
     mbar_init(q_full, 1);
@@ -291,21 +294,33 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         commit(drained);
         mbar_drain(drained, 0);
       }
-    } else if (warp == 10 && n > 0 && (masked || keys < a.p.Lk)) {
+    } else if (warp == 10 && n > 0 && fixes) {
       // ---- key mask, values that may not be attended ---------------------------------------------------------------
       const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
       bool ok = true;
-      int slot = pair && n > 1 ? 2 : 1;  // ring slot of the values of tile t: the keys loaded ahead come before
+      int slot = 0;
+      const auto follow = [&]() {  // the next stage of the ring, once it is loaded
+        const int s = slot % kStages;
+        ok = ok && warp_wait(full(s), (slot / kStages) & 1, bail);
+        ++slot;
+        return s;
+      };
+      const auto release = [&](int s) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
+      };
+      release(follow());
+      if (pair && n > 1) release(follow());
       const int ahead = pair ? 2 : 1;
       for (int t = 0; t < n && ok; ++t) {
-        const int s = slot % kStages, round = slot / kStages;
-        slot += t + ahead < n ? 2 : 1;
-        if (!needs_fix(t)) continue;
-        uint32_t word[4];
+        uint32_t word[4] = {kFull, kFull, kFull, kFull};
+        const bool fix = needs_fix(t);
+        if (fix) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = (t0 + t) * 128 + 32 * i + lane;
-          word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
+          for (int i = 0; i < 4; ++i) {
+            const int j = (t0 + t) * 128 + 32 * i + lane;
+            word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
+          }
         }
         if (masked) {
           const int m = t % kMaskRing;
@@ -315,20 +330,27 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           __syncwarp();
           if (lane == 0) mbar_arrive(m_full(m));
         }
-        ok = warp_wait(full(s), round & 1, bail);
+        const int s = follow();
         if (!ok) break;
-        if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
-          // a row's 128 bytes: eight lanes, four rows at a time (the swizzle permutes within the row, zeros do not care)
-          for (int r = lane >> 3; r < 128; r += 4) {
-            const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
-            if ((w >> (r & 31)) & 1) continue;
-            for (int x = 0; x < NSUB; ++x)
-              smem_zero16(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16);
+        if (fix) {
+          if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
+            // a row's 128 bytes: eight lanes, four rows at a time (the swizzle permutes within the row, zeros do not care)
+            for (int r = lane >> 3; r < 128; r += 4) {
+              const uint32_t w = r < 32 ? word[0] : r < 64 ? word[1] : r < 96 ? word[2] : word[3];
+              if ((w >> (r & 31)) & 1) continue;
+              for (int x = 0; x < NSUB; ++x) smem_zero16(s_ring + s * kStageBytes + x * kTileBytes + r * 128 + (lane & 7) * 16);
+            }
+            fence_async_smem();
           }
-          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(fixed(s));
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(fixed(s));
+        release(s);
+        if (t + ahead < n) {
+          const int sk = follow();
+          if (!ok) break;
+          release(sk);
+        }
       }
     }
   } else {

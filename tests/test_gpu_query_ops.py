@@ -76,18 +76,18 @@ LONG = [(40, 1, 2500, 8, 4, 64), (40, 3, 1900, 4, 4, 128), (2, 1500, 2700, 16, 8
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("shape", LONG, ids=lambda s: "x".join(map(str, s)))
-@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("masked", ["none", "lengths", "mask", "both"])
 def test_attention_of_many_tiles(cuda_device, shape, dtype, masked):
     B, Lq, Lk, Hq, Hkv, D = shape
     q, k, v = _rand((B, Lq, Hq, D), dtype, 1), _rand((B, Lk, Hkv, D), dtype, 2), _rand((B, Lk, Hkv, D), dtype, 3)
     dout = _rand((B, Lq, Hq, D), dtype, 4)
     g = torch.Generator(device="cuda").manual_seed(5)
-    lengths = torch.randint(Lk // 2, Lk + 1, (B,), generator=g, device="cuda") if masked else None
-    mask = torch.rand(B, Lk, generator=g, device="cuda") < 0.8 if masked else None
+    lengths = torch.randint(Lk // 2, Lk + 1, (B,), generator=g, device="cuda") if masked in ("lengths", "both") else None
+    mask = torch.rand(B, Lk, generator=g, device="cuda") < 0.8 if masked in ("mask", "both") else None
     got = _run(q, k, v, dout, key_lengths=lengths, key_mask=mask)
     for b in range(0, B, 19):  # the float64 form sample by sample
         one = slice(b, b + 1)
-        ok = R.allowed(1, Lk, lengths[one] if masked else None, mask[one] if masked else None)
+        ok = R.allowed(1, Lk, None if lengths is None else lengths[one], None if mask is None else mask[one])
         _compare({n: t[one] for n, t in got.items()}, R.attention(q[one], k[one], v[one], ok, 1 / math.sqrt(D), dout[one]))
 
 
