@@ -438,20 +438,14 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   }
 }
 
-// g[i] = f * (sum of the parts in order); four elements a thread
+// g[i] = f * (sum of the parts in order)
 template <typename T>
 __global__ void __launch_bounds__(256) att_sum_kernel(const float* __restrict__ part, int splits, long long count, float f, T* __restrict__ g) {
   grid_dependency_wait();
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (long long)gridDim.x * 1024) {
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < splits; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(part + k * count + i);
-      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
-    }
-    uint2 w;
-    w.x = pack2<T>(s.x * f, s.y * f);
-    w.y = pack2<T>(s.z * f, s.w * f);
-    *reinterpret_cast<uint2*>(g + i) = w;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int k = 0; k < splits; ++k) s += part[k * count + i];
+    g[i] = from_float<T>(s * f);
   }
 }
 

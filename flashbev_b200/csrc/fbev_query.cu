@@ -12,6 +12,7 @@
 #include "fbev_attention.cuh"
 #include "fbev_attention_tc.cuh"
 #include "fbev_attention_grad_tc.cuh"
+#include "fbev_attention_split_tc.cuh"
 #include "fbev_norm.cuh"
 #include "fbev_rotary.cuh"
 
@@ -54,9 +55,9 @@ static bool tma_operand(const void* ptr, const int64_t (&stride)[3], const int64
   return true;
 }
 
-// 16-bit types whose rows TMA can address: heads of whole 16 bytes, strides of whole 16 bytes.  Everything else takes the
-// one-warp-per-row kernels.
-static bool on_tensor_cores(const FbevAttention& p) {
+// 16-bit types whose rows TMA can address: heads of whole 16 bytes, strides of whole 16 bytes.  Everything else goes through
+// the kernels of three-part operands.
+static bool direct(const FbevAttention& p) {
   if (p.dtype == FBEV_F32 || p.D % 8 != 0 || p.Lk == 0 || p.Lq == 0 || p.B == 0 || p.Hq / p.Hkv > 128) return false;
   return tma_operand(p.q, p.q_stride, {p.B, p.Lq, p.Hq}, p.q_shared != 0) &&
          tma_operand(p.k, p.k_stride, {p.B, p.Lk, p.Hkv}, false) && tma_operand(p.v, p.v_stride, {p.B, p.Lk, p.Hkv}, false);
@@ -82,8 +83,69 @@ static AttPlan attention_plan(const FbevAttention& p) {
 static size_t split_output_bytes(const FbevAttention& p, const AttPlan& pl) {
   return round_up((size_t)pl.splits * p.B * p.Hkv * att_rows(p) * p.D * 4, 256);
 }
+// ---- three-part operands ----------------------------------------------------------------------------------------------
+
+struct SplitPlan {
+  int x_tiles, y_tiles, x_rows, splits, per_split;
+};
+static SplitPlan split_plan(const FbevAttention& p, int mode) {
+  const bool key_rows = mode == kSplitDv || mode == kSplitDk;
+  SplitPlan pl;
+  const int row_tiles = (int)((att_rows(p) + 127) / 128), key_tiles = (p.Lk + 127) / 128;
+  pl.x_tiles = key_rows ? key_tiles : row_tiles;
+  pl.y_tiles = key_rows ? row_tiles : key_tiles;
+  pl.x_rows = key_rows ? p.Lk : (int)att_rows(p);
+  const long long blocks = (long long)p.B * p.Hkv * pl.x_tiles;
+  long long splits = blocks > 0 && blocks < kSms ? kSms / blocks : 1;
+  if (splits > pl.y_tiles) splits = pl.y_tiles > 0 ? pl.y_tiles : 1;
+  pl.per_split = (int)((pl.y_tiles + splits - 1) / splits);
+  if (pl.per_split < 1) pl.per_split = 1;
+  pl.splits = (pl.y_tiles + pl.per_split - 1) / pl.per_split;
+  if (pl.splits < 1) pl.splits = 1;
+  return pl;
+}
+
+// Offsets in the workspace.  The parts of one result are summed before the next is computed and share their place.
+struct SplitLayout {
+  int width;
+  size_t q, k, v, go, allowed, nlse, ndelta, part, part_lse, bytes;
+};
+static SplitLayout split_layout(const FbevAttention& p, bool backward) {
+  SplitLayout l{};
+  l.width = (p.D + 7) / 8 * 8;
+  const size_t heads = (size_t)p.B * p.Hkv, rows = heads * att_rows(p), keys = heads * p.Lk;
+  const size_t row_bytes = round_up(rows * 3 * l.width * 2, 256), key_bytes = round_up(keys * 3 * l.width * 2, 256);
+  const size_t stat = round_up(heads * ((att_rows(p) + 127) / 128) * 512, 256);
+  size_t at = 0;
+  const auto take = [&](size_t n) {
+    const size_t here = at;
+    at += n;
+    return here;
+  };
+  l.q = take(row_bytes);
+  l.k = take(key_bytes);
+  l.v = take(key_bytes);
+  l.allowed = take(round_up((size_t)p.B * ((p.Lk + 127) / 128) * 512, 256));
+  size_t part = 0;
+  if (backward) {
+    l.go = take(row_bytes);
+    l.nlse = take(stat);
+    l.ndelta = take(stat);
+  }
+  for (int mode = backward ? kSplitDv : kSplitOut; mode <= (backward ? kSplitDk : kSplitOut); ++mode) {
+    const SplitPlan pl = split_plan(p, mode);
+    if (pl.splits == 1 && p.dtype == FBEV_F32) continue;
+    const size_t n = (size_t)pl.splits * (mode == kSplitDv || mode == kSplitDk ? keys : rows) * p.D * 4;
+    if (n > part) part = n;
+  }
+  l.part = take(round_up(part, 256));
+  if (!backward && part > 0) l.part_lse = take(round_up((size_t)split_plan(p, kSplitOut).splits * heads * att_rows_padded(p) * 4, 256));
+  l.bytes = at;
+  return l;
+}
+
 static size_t forward_workspace(const FbevAttention& p) {
-  if (!on_tensor_cores(p)) return 0;
+  if (!direct(p)) return split_layout(p, false).bytes;
   const AttPlan pl = attention_plan(p);
   if (pl.splits == 1) return 0;
   return split_output_bytes(p, pl) + round_up((size_t)pl.splits * p.B * p.Hkv * att_rows_padded(p) * 4, 256);
@@ -180,6 +242,149 @@ static float score_factor(const FbevAttention& p) {
   return c < 1e-30f ? 1e-30f : c;
 }
 
+// ---- three-part operands: launches -------------------------------------------------------------------------------------
+
+static int encode_parts(CUtensorMap* map, const void* ptr, long long rows, long long heads, int width) {
+  const EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return FBEV_ERR_NO_DEVICE;
+  const cuuint64_t d[4] = {(cuuint64_t)width, (cuuint64_t)rows, 3, (cuuint64_t)heads};
+  const cuuint64_t st[3] = {(cuuint64_t)width * 6, (cuuint64_t)width * 2, (cuuint64_t)rows * width * 6};
+  const cuuint32_t box[4] = {64, 128, 3, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult rc = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), d, st, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+
+template <typename T>
+static int split_operands(const FbevAttention& p, const SplitLayout& l, const T* out, const float* lse, const T* go, cudaStream_t st) {
+  char* ws = reinterpret_cast<char*>(p.workspace);
+  const int G = p.Hq / p.Hkv;
+  SplitSet set{};
+  const auto fill = [&](int i, const void* src, const int64_t* stride, int g, int len, int shared, size_t at) {
+    SplitSource& s = set.of[i];
+    s.src = src;
+    for (int k = 0; k < 3; ++k) s.stride[k] = stride[k];
+    s.G = g;
+    s.L = len;
+    s.shared = shared;
+    s.parts = reinterpret_cast<__nv_bfloat16*>(ws + at);
+    s.width = l.width;
+  };
+  const int64_t go_stride[3] = {(int64_t)p.Lq * p.Hq * p.D, (int64_t)p.Hq * p.D, p.D};
+  fill(0, p.q, p.q_stride, G, p.Lq, p.q_shared, l.q);
+  fill(1, p.k, p.k_stride, 1, p.Lk, 0, l.k);
+  fill(2, p.v, p.v_stride, 1, p.Lk, 0, l.v);
+  set.of[1].allowed = set.of[2].allowed = reinterpret_cast<float*>(ws + l.allowed);  // both clear, both write the same flags
+  int count = 3;
+  if (go != nullptr) {
+    fill(3, go, go_stride, G, p.Lq, 0, l.go);
+    set.of[3].out = out;
+    set.of[3].lse = lse;
+    set.of[3].nlse = reinterpret_cast<float*>(ws + l.nlse);
+    set.of[3].ndelta = reinterpret_cast<float*>(ws + l.ndelta);
+    count = 4;
+  }
+  long long blocks = 0;
+  for (int i = 0; i < 4; ++i) {
+    set.first[i] = (unsigned)blocks;
+    if (i < count) blocks += (long long)p.B * p.Hkv * (((long long)set.of[i].L * set.of[i].G + 127) / 128) * 16;
+    if (blocks >= (1ll << 31)) return FBEV_ERR_RANGE;
+    set.first[i + 1] = (unsigned)blocks;
+  }
+  split_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(p, set);
+  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+
+template <int NC, int MODE>
+static int split_launch(const FbevAttention& p, const SplitLayout& l, const SplitPlan& pl, float* g, float* part, float* lse, cudaStream_t st) {
+  static std::atomic<uint64_t> granted{0};
+  char* ws = reinterpret_cast<char*>(p.workspace);
+  const long long heads = (long long)p.B * p.Hkv, rows = att_rows(p);
+  CUtensorMap q, k, v, go;
+  int rc = allow_smem(att_split_kernel<NC, MODE>, kSplitSmem, granted);
+  if (rc == FBEV_OK) rc = encode_parts(&q, ws + l.q, rows, heads, l.width);
+  if (rc == FBEV_OK) rc = encode_parts(&k, ws + l.k, p.Lk, heads, l.width);
+  if (rc == FBEV_OK) rc = encode_parts(&v, ws + l.v, p.Lk, heads, l.width);
+  if (rc == FBEV_OK) rc = MODE == kSplitOut ? FBEV_OK : encode_parts(&go, ws + l.go, rows, heads, l.width);
+  if (rc != FBEV_OK) return rc;
+  if (MODE == kSplitOut) go = q;
+  SplitArgs a;
+  const bool key_rows = MODE == kSplitDv || MODE == kSplitDk;
+  a.x0 = key_rows ? k : q;
+  a.y0 = key_rows ? q : k;
+  a.x1 = key_rows ? v : go;
+  a.y1 = key_rows ? go : v;
+  a.z = MODE == kSplitOut ? v : MODE == kSplitDv ? go : MODE == kSplitDq ? k : q;
+  a.p = p;
+  a.x_tiles = pl.x_tiles;
+  a.y_tiles = pl.y_tiles;
+  a.x_rows = pl.x_rows;
+  a.splits = pl.splits;
+  a.per_split = pl.per_split;
+  a.allowed = reinterpret_cast<const float*>(ws + l.allowed);
+  a.nlse = reinterpret_cast<const float*>(ws + l.nlse);
+  a.ndelta = reinterpret_cast<const float*>(ws + l.ndelta);
+  a.g = g;
+  a.lse = lse;
+  a.part = part;
+  a.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
+  a.c = score_factor(p);
+  launch_next(att_split_kernel<NC, MODE>, (unsigned)(heads * pl.x_tiles * pl.splits), kAttThreads, kSplitSmem, st, a);
+  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+
+// float32 results of one block per tile are written in place; all others pass through parts
+template <typename T, int MODE>
+static int split_result(const FbevAttention& p, const SplitLayout& l, T* g, float* lse, cudaStream_t st) {
+  const SplitPlan pl = split_plan(p, MODE);
+  const bool whole = pl.splits == 1 && std::is_same<T, float>::value;
+  float* part = whole ? nullptr : reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + l.part);
+  float* into = reinterpret_cast<float*>(whole ? g : nullptr);
+  const int rc = p.D <= 64 ? split_launch<1, MODE>(p, l, pl, into, part, lse, st) : split_launch<2, MODE>(p, l, pl, into, part, lse, st);
+  if (rc != FBEV_OK || whole) return rc;
+  if (MODE == kSplitOut) {
+    launch_next(att_join_kernel<T>, (unsigned)((att_rows(p) * p.B * p.Hkv + 3) / 4), 128, 0, st, p, (const float*)part,
+                (const float*)reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + l.part_lse), pl.splits, g, lse);
+  } else {
+    const bool key_rows = MODE == kSplitDv || MODE == kSplitDk;
+    const long long count = (long long)p.B * (key_rows ? (long long)p.Lk * p.Hkv : (long long)p.Lq * p.Hq) * p.D;
+    const long long want = (count + 255) / 256;
+    launch_next(att_sum_kernel<T>, (unsigned)(want < kSms * 8 ? want : kSms * 8), 256, 0, st, (const float*)part, pl.splits, count,
+                MODE == kSplitDv ? 1.0f : p.scale, g);
+  }
+  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+}
+
+static int clear(void* ptr, size_t bytes, cudaStream_t st) {
+  if (ptr == nullptr || bytes == 0 || cudaMemsetAsync(ptr, 0, bytes, st) == cudaSuccess) return FBEV_OK;
+  cudaGetLastError();
+  return FBEV_ERR_LAUNCH;
+}
+
+template <typename T>
+static int split_forward(const FbevAttention& p, T* out, float* lse, cudaStream_t st) {
+  if (p.Lk == 0) return clear(out, (size_t)p.B * att_rows(p) * p.Hkv * p.D * sizeof(T), st);
+  const SplitLayout l = split_layout(p, false);
+  const int rc = split_operands<T>(p, l, nullptr, nullptr, nullptr, st);
+  return rc != FBEV_OK ? rc : split_result<T, kSplitOut>(p, l, out, lse, st);
+}
+
+template <typename T>
+static int split_backward(const FbevAttention& p, const T* out, const float* lse, const T* go, T* gq, T* gk, T* gv, cudaStream_t st) {
+  if (p.Lq == 0 || p.Lk == 0) {
+    const size_t rows = (size_t)p.B * att_rows(p) * p.Hkv * p.D * sizeof(T), keys = (size_t)p.B * p.Lk * p.Hkv * p.D * sizeof(T);
+    int rc = clear(gq, rows, st);
+    if (rc == FBEV_OK) rc = clear(gk, keys, st);
+    return rc == FBEV_OK ? clear(gv, keys, st) : rc;
+  }
+  const SplitLayout l = split_layout(p, true);
+  int rc = split_operands<T>(p, l, out, lse, go, st);
+  if (rc == FBEV_OK && gq) rc = split_result<T, kSplitDq>(p, l, gq, nullptr, st);
+  if (rc == FBEV_OK && gk) rc = split_result<T, kSplitDv>(p, l, gv, nullptr, st);
+  if (rc == FBEV_OK && gk) rc = split_result<T, kSplitDk>(p, l, gk, nullptr, st);
+  return rc;
+}
+
 template <typename T, int NSUB>
 static int tensor_forward(const FbevAttention& p, T* out, float* lse, cudaStream_t st) {
   static std::atomic<uint64_t> granted{0};
@@ -207,12 +412,10 @@ static int tensor_forward(const FbevAttention& p, T* out, float* lse, cudaStream
 template <typename T>
 static int attention_forward(const FbevAttention& p, T* out, float* lse, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (on_tensor_cores(p) && (uintptr_t)out % 16 == 0)
+    if (direct(p))
       return p.D <= 64 ? tensor_forward<T, 1>(p, out, lse, st) : tensor_forward<T, 2>(p, out, lse, st);
   }
-  const long long units = att_rows(p) * p.B * p.Hkv;
-  att_row_kernel<T><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(p, out, lse);
-  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+  return split_forward<T>(p, out, lse, st);
 }
 
 // blocks along the other side when this side's tiles leave SMs idle
@@ -235,16 +438,14 @@ static size_t gradient_part_bytes(const FbevAttention& p, bool kv) {  // of one 
   if (pl.splits == 1) return 0;
   return round_up((size_t)pl.splits * p.B * (kv ? (size_t)p.Lk * p.Hkv : (size_t)p.Lq * p.Hq) * p.D * 4, 256);
 }
-static size_t delta_bytes(const FbevAttention& p) { return round_up((size_t)p.B * p.Hkv * att_rows_padded(p) * 4, 256); }
 static size_t stat_bytes(const FbevAttention& p) {  // -lse or -delta by row tile
   return (size_t)p.B * p.Hkv * gradient_plan(p, false).row_tiles * 512;
 }
-// both statistics, then the parts of dQ, and after those are summed the parts of dK and dV in the same place; room for the
-// delta of the row kernels too, which take over when an address of the gradients is not aligned
+// both statistics, then the parts of dQ, and after those are summed the parts of dK and dV in the same place
 static size_t backward_workspace(const FbevAttention& p) {
-  if (!on_tensor_cores(p)) return delta_bytes(p);
+  if (!direct(p)) return split_layout(p, true).bytes;
   const size_t q = gradient_part_bytes(p, false), kv = 2 * gradient_part_bytes(p, true);
-  return delta_bytes(p) + 2 * stat_bytes(p) + (q > kv ? q : kv);
+  return 2 * stat_bytes(p) + (q > kv ? q : kv);
 }
 
 template <typename T, int NSUB, bool KV>
@@ -275,7 +476,7 @@ static int tensor_gradient(const FbevAttention& p, const T* go, T* g0, T* g1, cu
   launch_next(att_grad_kernel<T, NSUB, KV>, (unsigned)blocks, kAttThreads, AttGradShape<NSUB>::kSmem, st, a);
   if (a.pl.splits > 1) {
     const long long count = (long long)p.B * (KV ? (long long)p.Lk * p.Hkv : (long long)p.Lq * p.Hq) * p.D;
-    const long long want = (count / 4 + 255) / 256;
+    const long long want = (count + 255) / 256;
     const unsigned grid = (unsigned)(want < kSms * 8 ? want : kSms * 8);
     launch_next(att_sum_kernel<T>, grid, 256, 0, st, (const float*)a.part0, a.pl.splits, count, p.scale, g0);
     if (KV) launch_next(att_sum_kernel<T>, grid, 256, 0, st, (const float*)a.part1, a.pl.splits, count, 1.0f, g1);
@@ -300,16 +501,10 @@ template <typename T>
 static int attention_backward(const FbevAttention& p, const T* out, const float* lse, const T* go, T* gq, T* gk, T* gv,
                               cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    const uintptr_t all = (uintptr_t)out | (uintptr_t)go | (uintptr_t)gq | (uintptr_t)gk | (uintptr_t)gv;
-    if (on_tensor_cores(p) && all % 16 == 0)
+    if (direct(p))
       return p.D <= 64 ? tensor_backward<T, 1>(p, out, lse, go, gq, gk, gv, st) : tensor_backward<T, 2>(p, out, lse, go, gq, gk, gv, st);
   }
-  float* delta = reinterpret_cast<float*>(p.workspace);
-  const long long units = att_rows(p) * p.B * p.Hkv, keys = (long long)p.B * p.Lk * p.Hkv;
-  if (units > 0) att_delta_kernel<T><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(p, out, go, delta);
-  if (gq && units > 0) att_row_grad_q_kernel<T><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(p, lse, delta, go, gq);
-  if (gk && keys > 0) att_row_grad_kv_kernel<T><<<(unsigned)((keys + 3) / 4), 128, 0, st>>>(p, lse, delta, go, gk, gv);
-  return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
+  return split_backward<T>(p, out, lse, go, gq, gk, gv, st);
 }
 
 }  // namespace fbev
@@ -340,7 +535,7 @@ int fbev_cross_attention(const FbevAttention* p, void* out, float* lse, void* st
   if (rc != FBEV_OK) return rc;
   if (p->B == 0 || p->Lq == 0) return FBEV_OK;
   if (out == nullptr || !has_pointers(p)) return FBEV_ERR_NULL;
-  if ((uintptr_t)out % size_of(p->dtype) || (uintptr_t)lse % 16) return FBEV_ERR_ALIGN;
+  if ((uintptr_t)out % 16 || (uintptr_t)lse % 16) return FBEV_ERR_ALIGN;
   rc = check_workspace(p, 0);
   if (rc != FBEV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -360,7 +555,7 @@ int fbev_cross_attention_grad(const FbevAttention* p, const void* out, const flo
   const bool queries = p->Lq > 0;
   if (!has_pointers(p) || (queries && (!out || !lse || !grad_out))) return FBEV_ERR_NULL;
   const uintptr_t all = (uintptr_t)out | (uintptr_t)grad_out | (uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v;
-  if (all % size_of(p->dtype) || (uintptr_t)lse % 16) return FBEV_ERR_ALIGN;
+  if (all % 16 || (uintptr_t)lse % 16) return FBEV_ERR_ALIGN;
   rc = check_workspace(p, 1);
   if (rc != FBEV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

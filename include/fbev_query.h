@@ -55,12 +55,12 @@ size_t fbev_cross_attention_lse_count(const FbevAttention* p);
 /* Device bytes of workspace for the forward (backward = 0) or the backward (backward = 1); 0 for an invalid problem. */
 size_t fbev_cross_attention_workspace_bytes(const FbevAttention* p, int backward);
 
-/* out: device, contiguous [B,Lq,Hq,D].  lse: device, 16-byte aligned, fbev_cross_attention_lse_count() floats for the
+/* out: device, contiguous [B,Lq,Hq,D], 16-byte aligned.  lse: device, 16-byte aligned, fbev_cross_attention_lse_count() floats for the
  * backward, or NULL. */
 int fbev_cross_attention(const FbevAttention* p, void* out, float* lse, void* stream);
 
 /* Gradients of sum(out * grad_out).  out, grad_out: contiguous [B,Lq,Hq,D]; lse: as the forward left it.
- * grad_q [B,Lq,Hq,D], grad_k and grad_v [B,Lk,Hkv,D], contiguous, overwritten; grad_q, or grad_k and grad_v together,
+ * grad_q [B,Lq,Hq,D], grad_k and grad_v [B,Lk,Hkv,D], contiguous, overwritten; all 16-byte aligned; grad_q, or grad_k and grad_v together,
  * may be NULL.  The results do not depend on the order in which blocks run. */
 int fbev_cross_attention_grad(const FbevAttention* p, const void* out, const float* lse, const void* grad_out,
                               void* grad_q, void* grad_k, void* grad_v, void* stream);
