@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   extern __shared__ unsigned char s_raw[];
   __shared__ __align__(8) uint64_t s_bar[3 * kStages + 7 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
+  __shared__ __align__(16) float s_stat[KV ? kMaskRing : 1][2][128];  // -lse and -delta of the row tiles ahead
   __shared__ uint32_t s_tmem;
   __shared__ int s_bail;
 
@@ -296,6 +297,19 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         if (!ok) break;
         release(s1);
       }
+    } else if (KV && warp == 10 && n > 0) {
+      // ---- statistics of the row tiles -----------------------------------------------------------------------------
+      const float4* nlse = reinterpret_cast<const float4*>(a.nlse + ((long long)bg * pl.row_tiles + t0) * 128);
+      const float4* ndelta = reinterpret_cast<const float4*>(a.ndelta + ((long long)bg * pl.row_tiles + t0) * 128);
+      for (int t = 0; t < n; ++t) {
+        const int m = t % kMaskRing;
+        const float4 l = nlse[32 * t + lane], d = ndelta[32 * t + lane];
+        if (t >= kMaskRing && !warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail)) break;
+        *reinterpret_cast<float4*>(&s_stat[m][0][4 * lane]) = l;
+        *reinterpret_cast<float4*>(&s_stat[m][1][4 * lane]) = d;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m_full(m));
+      }
     }
   } else {
     // ---- P and dS ----------------------------------------------------------------------------------------------------
@@ -306,9 +320,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     const long long row = (long long)xt * tile_rows + r;             // dQ
     const bool row_live = !KV && r < tile_rows && row < rows;
     const int key = xt * 128 + r;                                    // dK, dV
-    const float* nlse = a.nlse + ((long long)bg * pl.row_tiles + (KV ? t0 : xt)) * 128;
-    const float* ndelta = a.ndelta + ((long long)bg * pl.row_tiles + (KV ? t0 : xt)) * 128;
-    const float nl = KV ? 0.0f : nlse[r], nd = KV ? 0.0f : ndelta[r];
+    const float nl = KV ? 0.0f : a.nlse[((long long)bg * pl.row_tiles + xt) * 128 + r];
+    const float nd = KV ? 0.0f : a.ndelta[((long long)bg * pl.row_tiles + xt) * 128 + r];
     bool ok = true;
     for (int t = 0; t < n; ++t) {
       const int mr = t % kMaskRing;
@@ -327,6 +340,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       }
       const bool cut = (word[0] & word[1]) != kFull;
       ok = warp_wait(s_full, t & 1, bail);
+      if (ok && KV) ok = warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
       if (!ok) break;
       tc_fence_after();
       float p[64];
@@ -341,13 +355,14 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
 #pragma unroll
       for (int x = 0; x < 64; x += 4) {
         float4 l = make_float4(nl, nl, nl, nl);
-        if (KV) l = *reinterpret_cast<const float4*>(nlse + 128 * t + 64 * h + x);
+        if (KV) l = *reinterpret_cast<const float4*>(&s_stat[mr][0][64 * h + x]);
         const float2 e0 = fma2(make_float2(p[x], p[x + 1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
         const float2 e1 = fma2(make_float2(p[x + 2], p[x + 3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
-        p[x] = exp2_fast(e0.x);
-        p[x + 1] = exp2_fast(e0.y);
-        p[x + 2] = exp2_fast(e1.x);
-        p[x + 3] = exp2_fast(e1.y);
+        const float2 q0 = exp2_pair<FBEV_POLY_GRAD>(e0, x / 2), q1 = exp2_pair<FBEV_POLY_GRAD>(e1, x / 2 + 1);
+        p[x] = q0.x;
+        p[x + 1] = q0.y;
+        p[x + 2] = q1.x;
+        p[x + 3] = q1.y;
       }
       if (KV) {
         uint32_t packed[32];
@@ -371,7 +386,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
 #pragma unroll
         for (int x = 0; x < 32; x += 4) {
           float4 d = make_float4(nd, nd, nd, nd);
-          if (KV) d = *reinterpret_cast<const float4*>(ndelta + 128 * t + 64 * h + 32 * y + x);
+          if (KV) d = *reinterpret_cast<const float4*>(&s_stat[mr][1][64 * h + 32 * y + x]);
           const float* q = p + 32 * y + x;
           float2 s0 = add2(make_float2(dp[x], dp[x + 1]), make_float2(d.x, d.y));
           float2 s1 = add2(make_float2(dp[x + 2], dp[x + 3]), make_float2(d.z, d.w));
@@ -391,7 +406,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_done);
+      if (lane == 0) {
+        mbar_arrive(ds_done);
+        if (KV) mbar_arrive(m_empty(mr));
+      }
     }
     if (ok && n > 0) ok = warp_wait(acc_full, 0, bail);
     tc_fence_after();

@@ -52,6 +52,36 @@ struct AttFwdShape {
   static constexpr uint32_t kSmem = 2 * kStageBytes + kStages * kStageBytes + 1024;
 };
 
+// 2^x of two numbers on the multiply-add pipe, for weights that are rounded to 16 bits: x = n + f with n whole and
+// |f| <= 1/2, 2^f by the cubic with the least largest relative error on that interval (2^-13.7, Remez exchange), n added to
+// the exponent.  The unit for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with
+// the rest of the softmax; a part of the weights goes this way instead.  What is below 2^-126 becomes 2^-126: a score of
+// -infinity leaves a weight that no sum notices, and rows without any key are told by their maximum.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x = make_float2(max_nan(x.x, -126.0f), max_nan(x.y, -126.0f));
+  const float2 r = add2(x, make_float2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: the whole part in the low bits
+  const float2 n = add2(r, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
+  p = fma2(p, f, make_float2(0.69326097f, 0.69326097f));
+  p = fma2(p, f, make_float2(0.99992806f, 0.99992806f));
+  return make_float2(__uint_as_float((__float_as_uint(r.x) << 23) + __float_as_uint(p.x)),
+                     __uint_as_float((__float_as_uint(r.y) << 23) + __float_as_uint(p.y)));
+}
+
+// pair i of a run of weights: this many of eight on the multiply-add pipe
+#ifndef FBEV_POLY_FWD
+#define FBEV_POLY_FWD 3
+#endif
+#ifndef FBEV_POLY_GRAD
+#define FBEV_POLY_GRAD 3
+#endif
+template <int OF8>
+__device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
+  if ((i * OF8) % 8 < OF8) return exp2_poly(x);
+  return make_float2(exp2_fast(x.x), exp2_fast(x.y));
+}
+
 constexpr int kMaskRing = 4;
 constexpr int kAttThreads = 384;
 
@@ -428,7 +458,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
 #pragma unroll
         for (int x = 0; x < 64; ++x) {
           const float2 e = fma2(make_float2(s[2 * x], s[2 * x + 1]), make_float2(a.c, a.c), make_float2(off, off));
-          const float2 pr = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+          const float2 pr = exp2_pair<FBEV_POLY_FWD>(e, x);
           part[x & 3] = add2(part[x & 3], pr);
           packed[x] = pack2<T>(pr.x, pr.y);
         }
@@ -476,7 +506,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         sum = sum * f0 + sum1 * f1;
         m = mm;
       }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const bool none = m == -INFINITY;  // no key
+      const float inv = none ? 0.0f : 1.0f / sum;
       const bool parted = pl.splits > 1;
       const long long l = row / pl.G;
       T* dst = reinterpret_cast<T*>(a.out) + (((long long)b * a.p.Lq + l) * a.p.Hq + g * pl.G + (int)(row - l * pl.G)) * a.p.D;
@@ -510,9 +541,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       }
       if (live) {
         if (parted)
-          a.part_lse[at * att_rows_padded(a.p) + row] = sum == 0.0f ? -INFINITY : m + log2f(sum);
+          a.part_lse[at * att_rows_padded(a.p) + row] = none ? -INFINITY : m + log2f(sum);
         else if (a.lse != nullptr)
-          a.lse[(long long)bg * att_rows_padded(a.p) + row] = sum == 0.0f ? INFINITY : m + log2f(sum);
+          a.lse[(long long)bg * att_rows_padded(a.p) + row] = none ? INFINITY : m + log2f(sum);
       }
     }
     tc_fence_before();
