@@ -65,13 +65,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   __shared__ int s_bail;
 
   const AttGradPlan& pl = a.pl;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   int u = blockIdx.x;
   const int split = u % pl.splits;
   u /= pl.splits;
   const int x_tiles = KV ? pl.key_tiles : pl.row_tiles;
   const int xt = u % x_tiles, bg = u / x_tiles, b = bg / a.p.Hkv, g = bg % a.p.Hkv;
-  const int keys = att_keys(a.p, b);
+  const int keys = uniform(att_keys(a.p, b));
   const bool masked = a.p.key_mask != nullptr;
   const long long rows = att_rows(a.p);
   const int tile_rows = pl.TL * pl.G;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns of the SM are this block's
   const Bail bail{&s_bail, a.p.status};
   const uint32_t x_bytes = KV ? kStageBytes : (uint32_t)(NSUB * tile_rows * 128);
   const uint32_t y_bytes = KV ? (uint32_t)(NSUB * tile_rows * 128) : kStageBytes;
@@ -353,16 +353,22 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         if (lane == 0) mbar_arrive(p_done);
       }
 #pragma unroll
-      for (int x = 0; x < 64; x += 4) {
-        float4 l = make_float4(nl, nl, nl, nl);
-        if (KV) l = *reinterpret_cast<const float4*>(&s_stat[mr][0][64 * h + x]);
-        const float2 e0 = fma2(make_float2(p[x], p[x + 1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
-        const float2 e1 = fma2(make_float2(p[x + 2], p[x + 3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
-        const float2 q0 = exp2_pair<FBEV_POLY_GRAD>(e0, x / 2), q1 = exp2_pair<FBEV_POLY_GRAD>(e1, x / 2 + 1);
-        p[x] = q0.x;
-        p[x + 1] = q0.y;
-        p[x + 2] = q1.x;
-        p[x + 3] = q1.y;
+      for (int x = 0; x < 64; x += 16) {
+        float2 e[8];
+#pragma unroll
+        for (int y = 0; y < 8; y += 2) {
+          const float* q = p + x + 2 * y;
+          float4 l = make_float4(nl, nl, nl, nl);
+          if (KV) l = *reinterpret_cast<const float4*>(&s_stat[mr][0][64 * h + x + 2 * y]);
+          e[y] = fma2(make_float2(q[0], q[1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
+          e[y + 1] = fma2(make_float2(q[2], q[3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
+        }
+        exp2_run<FBEV_POLY_GRAD>(e);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          p[x + 2 * y] = e[y].x;
+          p[x + 2 * y + 1] = e[y].y;
+        }
       }
       if (KV) {
         uint32_t packed[32];
@@ -452,7 +458,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<512>(s_tmem);
   }
 }
 

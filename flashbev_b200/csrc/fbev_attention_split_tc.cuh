@@ -71,12 +71,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
   __shared__ uint32_t s_tmem;
   __shared__ int s_bail;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   int u = blockIdx.x;
   const int split = u % a.splits;
   u /= a.splits;
   const int xt = u % a.x_tiles, bg = u / a.x_tiles, b = bg / a.p.Hkv, g = bg % a.p.Hkv;
-  const int keys = att_keys(a.p, b);
+  const int keys = uniform(att_keys(a.p, b));
   const int t0 = split * a.per_split;
   int n = (kKeyRows ? (xt * 128 < keys ? a.y_tiles : 0) : (keys + 127) / 128) - t0;
   n = n < 0 ? 0 : n > a.per_split ? a.per_split : n;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns of the SM are this block's
   const Bail bail{&s_bail, a.p.status};
   grid_dependency_wait();  // the parts come from the kernels before
 
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<512>(s_tmem);
   }
 }
 

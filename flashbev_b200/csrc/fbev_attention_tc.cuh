@@ -8,8 +8,11 @@
 //   O += P V              P from tensor memory, V from shared memory (read across its rows), accumulator in tensor memory
 //
 // Roles: eight softmax warps (two groups of four, one per row tile), a warp that loads by TMA, a warp that issues the
-// matrix instructions, a warp that reads the key mask and clears values that may not be attended.  While one row tile is
-// in the hands of its softmax group the tensor cores work on the other.
+// matrix instructions, a warp that reads the key mask and clears values that may not be attended.  Step q of a block is key
+// tile q / 2 of row tile q % 2 (one row tile: q of that).  The scores of steps q + 1 .. q + kBufs - 1 are formed while a
+// softmax group works on step q; P V of step q and the scores of step q + kBufs, which take P's place, follow.  With heads
+// up to 64 wide tensor memory holds three score tiles, so a group finds its next one ready; with two it waits for both
+// products.
 //
 // m is the row's running maximum, raised only when a tile exceeds it by more than 8: weights then stay below 2^8 (no loss
 // in either type, both sides of the quotient carry the same factor) and the output, which lives in tensor memory, is
@@ -19,7 +22,7 @@
 // memory at the end.  Whenever the row tiles leave SMs without a block the key tiles are split over several blocks, which
 // leave normalised float32 outputs and their logarithmic sums for att_join_kernel.
 //
-// Tensor memory, columns: S/P of group 0 and 1 (128 each), O of group 0 and 1 (128 each).
+// Tensor memory, columns: S/P tiles from 0 (128 each), O of the two groups behind them (64 or 128 each).
 #pragma once
 #include "fbev_attention.cuh"
 #include "fbev_tc.cuh"
@@ -47,6 +50,8 @@ struct AttFwdArgs {
 
 template <int NSUB>
 struct AttFwdShape {
+  static constexpr int kBufs = NSUB == 1 ? 3 : 2;      // score tiles in tensor memory
+  static constexpr int kOutAt = 128 * kBufs, kOutCols = NSUB == 1 ? 64 : 128;
   static constexpr int kStages = NSUB == 1 ? 10 : 5;
   static constexpr uint32_t kStageBytes = NSUB * kTileBytes;
   static constexpr uint32_t kSmem = 2 * kStageBytes + kStages * kStageBytes + 1024;
@@ -57,29 +62,50 @@ struct AttFwdShape {
 // the exponent.  The unit for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with
 // the rest of the softmax; a part of the weights goes this way instead.  What is below 2^-126 becomes 2^-126: a score of
 // -infinity leaves a weight that no sum notices, and rows without any key are told by their maximum.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x = make_float2(max_nan(x.x, -126.0f), max_nan(x.y, -126.0f));
-  const float2 r = add2(x, make_float2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: the whole part in the low bits
-  const float2 n = add2(r, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-  float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
-  p = fma2(p, f, make_float2(0.69326097f, 0.69326097f));
-  p = fma2(p, f, make_float2(0.99992806f, 0.99992806f));
-  return make_float2(__uint_as_float((__float_as_uint(r.x) << 23) + __float_as_uint(p.x)),
-                     __uint_as_float((__float_as_uint(r.y) << 23) + __float_as_uint(p.y)));
-}
-
-// pair i of a run of weights: this many of eight on the multiply-add pipe
+// this many of eight pairs
 #ifndef FBEV_POLY_FWD
 #define FBEV_POLY_FWD 3
 #endif
 #ifndef FBEV_POLY_GRAD
 #define FBEV_POLY_GRAD 3
 #endif
+// eight pairs at once; the steps of the cubics side by side, the other exponentials between them
 template <int OF8>
-__device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
-  if ((i * OF8) % 8 < OF8) return exp2_poly(x);
-  return make_float2(exp2_fast(x.x), exp2_fast(x.y));
+__device__ __forceinline__ void exp2_run(float2 (&x)[8]) {
+  constexpr int K = OF8 > 0 ? OF8 : 1;
+  float2 r[K], f[K], p[K];
+  const auto unit = [&](int i) { x[i] = make_float2(exp2_fast(x[i].x), exp2_fast(x[i].y)); };
+  const auto between = [&](int stage) {  // pairs OF8 .. 7, spread over six stages
+#pragma unroll
+    for (int i = OF8; i < 8; ++i)
+      if ((i - OF8) * 6 / (8 - OF8) == stage) unit(i);
+  };
+  between(0);
+#pragma unroll
+  for (int i = 0; i < OF8; ++i) {
+    x[i] = make_float2(max_nan(x[i].x, -126.0f), max_nan(x[i].y, -126.0f));
+    r[i] = add2(x[i], make_float2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: the whole part in the low bits
+  }
+  between(1);
+#pragma unroll
+  for (int i = 0; i < OF8; ++i) {
+    const float2 n = add2(r[i], make_float2(-12582912.0f, -12582912.0f));
+    f[i] = fma2(n, make_float2(-1.0f, -1.0f), x[i]);
+  }
+  between(2);
+#pragma unroll
+  for (int i = 0; i < OF8; ++i) p[i] = fma2(f[i], make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
+  between(3);
+#pragma unroll
+  for (int i = 0; i < OF8; ++i) p[i] = fma2(p[i], f[i], make_float2(0.69326097f, 0.69326097f));
+  between(4);
+#pragma unroll
+  for (int i = 0; i < OF8; ++i) p[i] = fma2(p[i], f[i], make_float2(0.99992806f, 0.99992806f));
+  between(5);
+#pragma unroll
+  for (int i = 0; i < OF8; ++i)
+    x[i] = make_float2(__uint_as_float((__float_as_uint(r[i].x) << 23) + __float_as_uint(p[i].x)),
+                       __uint_as_float((__float_as_uint(r[i].y) << 23) + __float_as_uint(p[i].y)));
 }
 
 constexpr int kMaskRing = 4;
@@ -113,21 +139,22 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   constexpr int kStages = Shape::kStages;
   constexpr uint32_t kStageBytes = Shape::kStageBytes;
   extern __shared__ unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2 * kStages + kStages + 1 + 2 + 2 + 2 + 2 * kMaskRing + 1];
+  constexpr int kBufs = Shape::kBufs;
+  __shared__ __align__(8) uint64_t s_bar[3 * kStages + 3 * kBufs + 6 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
   __shared__ float s_stat[2][128];
   __shared__ uint32_t s_tmem;
   __shared__ int s_bail;
 
   const AttPlan& pl = a.pl;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // block -> (split, row block, sample, key head); row blocks of one key head are neighbours and share its keys in L2
   int u = blockIdx.x;
   const int split = u % pl.splits;
   u /= pl.splits;
   const int rb = u % pl.row_blocks;
   const int bg = u / pl.row_blocks, b = bg / a.p.Hkv, g = bg % a.p.Hkv;
-  const int keys = att_keys(a.p, b);
+  const int keys = uniform(att_keys(a.p, b));
   const int t0 = split * pl.per_split;
   int n = (keys + 127) / 128 - t0;  // key tiles of this block
   n = n < 0 ? 0 : n > pl.per_split ? pl.per_split : n;
@@ -143,13 +170,14 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
   const auto fixed = [&](int s) { return bars + 8 * (2 * kStages + s); };
-  const uint32_t q_full = bars + 8 * (3 * kStages);
-  const auto s_full = [&](int i) { return bars + 8 * (3 * kStages + 1 + i); };
-  const auto p_full = [&](int i) { return bars + 8 * (3 * kStages + 3 + i); };
-  const auto o_full = [&](int i) { return bars + 8 * (3 * kStages + 5 + i); };
-  const auto m_full = [&](int i) { return bars + 8 * (3 * kStages + 7 + i); };
-  const auto m_empty = [&](int i) { return bars + 8 * (3 * kStages + 7 + kMaskRing + i); };
-  const uint32_t drained = bars + 8 * (3 * kStages + 7 + 2 * kMaskRing);
+  const uint32_t q_full = bars + 8 * (3 * kStages), drained = q_full + 8;
+  const auto o_full = [&](int i) { return q_full + 16 + 8 * i; };  // the group's last product is done
+  const auto o_step = [&](int i) { return q_full + 32 + 8 * i; };  // ... each one
+  const auto s_full = [&](int i) { return q_full + 48 + 8 * i; };
+  const auto p_half = [&](int i) { return q_full + 48 + 8 * (kBufs + i); };
+  const auto p_full = [&](int i) { return q_full + 48 + 8 * (2 * kBufs + i); };
+  const auto m_full = [&](int i) { return q_full + 48 + 8 * (3 * kBufs + i); };
+  const auto m_empty = [&](int i) { return q_full + 48 + 8 * (3 * kBufs + kMaskRing + i); };
 
   // softmax warps with rows to work on: all four of a group, fewer when the only row tile is short
   const long long left = rows - (long long)(pair ? 0 : 2 * rb) * tile_rows;
@@ -167,9 +195,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
     }
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full(i), 1);
-      mbar_init(p_full(i), live_warps);
       mbar_init(o_full(i), 1);
+      mbar_init(o_step(i), 1);
+    }
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(s_full(i), 1);
+      mbar_init(p_half(i), live_warps);
+      mbar_init(p_full(i), live_warps);
     }
     for (int i = 0; i < kMaskRing; ++i) {
       mbar_init(m_full(i), 1);
@@ -183,10 +215,17 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns of the SM are this block's
   const Bail bail{&s_bail, a.p.status};
   // a tile whose values have to be cleared in places: masked, or cut off by the sample's length inside the tensor
   const auto needs_fix = [&](int t) { return masked || ((t0 + t + 1) * 128 > keys && keys < a.p.Lk); };
+
+  // steps, and which of them take a new tile of keys (the order of the ring: keys of the first kBufs steps, then the values
+  // of step q and the keys of step q + kBufs in turn)
+  const int streams = pair ? 2 : tiles, steps = pair ? n : n * tiles;
+  const auto tile_of = [&](int q) { return pair || streams == 1 ? q : q >> 1; };
+  const auto stream_of = [&](int q) { return streams == 1 ? 0 : q & 1; };
+  const auto new_tile = [&](int q) { return pair || streams == 1 || (q & 1) == 0; };
 
   if (warp >= 8) {
     set_registers_down<80>();
@@ -213,12 +252,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         __syncwarp();
         ++slot;
       };
-      load(&a.k, 0);
-      if (pair && n > 1) load(&a.k, 1);
-      const int ahead = pair ? 2 : 1;
-      for (int t = 0; t < n && ok; ++t) {
-        load(&a.v, t);
-        if (t + ahead < n) load(&a.k, t + ahead);
+      for (int q = 0; q < kBufs && q < steps; ++q)
+        if (new_tile(q)) load(&a.k, tile_of(q));
+      for (int q = 0; q < steps && ok; ++q) {
+        if (new_tile(q)) load(&a.v, tile_of(q));
+        if (q + kBufs < steps && new_tile(q + kBufs)) load(&a.k, tile_of(q + kBufs));
       }
       if (!ok) {
         // nothing may be left in flight when the block ends
@@ -244,26 +282,32 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         if (leader) umma_commit(bar);
         __syncwarp();
       };
-      const auto scores = [&](int i, int s) {
+      const auto scores = [&](int q, int s) {
         tc_fence_after();
         if (leader) {
+          const uint32_t d = tmem + 128 * (q % kBufs);
 #pragma unroll
           for (int x = 0; x < NSUB; ++x) {
-            const uint64_t da = desc_k_major(s_q + (pair ? 0 : i) * kStageBytes + x * kTileBytes);
+            const uint64_t da = desc_k_major(s_q + (pair ? 0 : stream_of(q)) * kStageBytes + x * kTileBytes);
             const uint64_t db = desc_k_major(s_ring + s * kStageBytes + x * kTileBytes);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (x * 4 + k < ksteps) umma_ss(tmem + 128 * i, da + 2 * k, db + 2 * k, i_s, x + k > 0);
+              if (x * 4 + k < ksteps) umma_ss(d, da + 2 * k, db + 2 * k, i_s, x + k > 0);
           }
+          umma_commit(s_full(q % kBufs));
         }
-        commit(s_full(i));
+        __syncwarp();
       };
-      const auto values = [&](int i, int s, bool first) {
+      const auto values = [&](int q, int s, int half, bool first) {  // half of the keys
         tc_fence_after();
         if (leader) {
           const uint64_t db = desc_mn_major(s_ring + s * kStageBytes);
+          const uint32_t d = tmem + Shape::kOutAt + Shape::kOutCols * stream_of(q), p = tmem + 128 * (q % kBufs);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) umma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, db + 128 * k, i_o, !first || k > 0);
+          for (int k = 0; k < 4; ++k) {
+            const int kk = 4 * half + k;
+            umma_ts(d, p + 8 * kk, db + 128 * kk, i_o, !first || kk > 0);
+          }
         }
         __syncwarp();
       };
@@ -272,53 +316,36 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         ok = ok && warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
         fix_parity ^= 1u << s;
       };
-      if (pair) {
-        for (int t = 0; t < 2 && t < n && ok; ++t) {
-          const int s = take();
-          if (!ok) break;
-          scores(t, s);
-          commit(empty(s));
+      int sk = 0, sv = 0;
+      const auto last_use = [&](int q) { return pair || streams == 1 || (q & 1) == 1; };  // of the tile of keys or values
+      for (int q = 0; q < kBufs && q < steps && ok; ++q) {
+        if (new_tile(q)) sk = take();
+        if (!ok) break;
+        scores(q, sk);
+        if (last_use(q)) commit(empty(sk));
+      }
+      for (int q = 0; q < steps && ok; ++q) {
+        const int i = stream_of(q), buf = q % kBufs, parity = (q / kBufs) & 1;
+        if (new_tile(q)) {
+          sv = take();
+          fix_wait(tile_of(q), sv);
         }
-        for (int t = 0; t < n && ok; ++t) {
-          const int i = t & 1, s = take();
-          fix_wait(t, s);
-          ok = ok && warp_wait(p_full(i), (t >> 1) & 1, bail);
-          if (!ok) break;
-          values(i, s, t < 2);
-          commit(empty(s));
-          if (t + 2 >= n) commit(o_full(i));
-          if (t + 2 < n) {
-            const int sk = take();
-            if (!ok) break;
-            scores(i, sk);
-            commit(empty(sk));
-          }
+        const bool more = q + kBufs < steps;
+        if (more && new_tile(q + kBufs)) sk = take();
+        ok = ok && warp_wait(p_half(buf), parity, bail);
+        if (!ok) break;
+        values(q, sv, 0, q < streams);
+        ok = warp_wait(p_full(buf), parity, bail);
+        if (!ok) break;
+        values(q, sv, 1, false);
+        if (more) scores(q + kBufs, sk);
+        if (leader) {
+          umma_commit(o_step(i));
+          if (q + streams >= steps) umma_commit(o_full(i));
+          if (last_use(q)) umma_commit(empty(sv));
+          if (more && last_use(q + kBufs)) umma_commit(empty(sk));
         }
-      } else {
-        const int sk0 = take();
-        if (ok) {
-          for (int i = 0; i < tiles; ++i) scores(i, sk0);
-          commit(empty(sk0));
-        }
-        for (int t = 0; t < n && ok; ++t) {
-          const int s = take();
-          fix_wait(t, s);
-          int sk = 0;
-          for (int i = 0; i < tiles; ++i) {
-            ok = ok && warp_wait(p_full(i), t & 1, bail);
-            if (!ok) break;
-            values(i, s, t == 0);
-            if (i == tiles - 1) commit(empty(s));
-            if (t + 1 == n) {
-              commit(o_full(i));
-              continue;
-            }
-            if (i == 0) sk = take();
-            if (!ok) break;
-            scores(i, sk);
-            if (i == tiles - 1) commit(empty(sk));
-          }
-        }
+        __syncwarp();
       }
       if (!ok) {
         commit(drained);
@@ -339,10 +366,19 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
       };
-      release(follow());
-      if (pair && n > 1) release(follow());
-      const int ahead = pair ? 2 : 1;
-      for (int t = 0; t < n && ok; ++t) {
+      for (int q = 0; q < kBufs && q < steps; ++q)
+        if (new_tile(q)) release(follow());
+      for (int q = 0; q < steps && ok; ++q) {
+        const bool keys_next = q + kBufs < steps && new_tile(q + kBufs);
+        if (!new_tile(q)) {
+          if (keys_next) {
+            const int sk = follow();
+            if (!ok) break;
+            release(sk);
+          }
+          continue;
+        }
+        const int t = tile_of(q);
         uint32_t word[4] = {kFull, kFull, kFull, kFull};
         const bool fix = needs_fix(t);
         if (fix) {
@@ -376,7 +412,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           if (lane == 0) mbar_arrive(fixed(s));
         }
         release(s);
-        if (t + ahead < n) {
+        if (keys_next) {
           const int sk = follow();
           if (!ok) break;
           release(sk);
@@ -389,7 +425,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
     const int i = warp >> 2, w4 = warp & 3;
     const int r = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)(w4 * 32) << 16);
-    const uint32_t t_s = lanes + 128 * i, t_o = lanes + 256 + 128 * i;
+    const uint32_t t_o = lanes + Shape::kOutAt + Shape::kOutCols * i;
     const int mine = pair ? (n - i + 1) / 2 : (i < tiles ? n : 0);  // key tiles of this group
     const bool works = w4 < live_warps && (pair || i < tiles);
     const int row_tile = pair ? 0 : 2 * rb + i;
@@ -400,7 +436,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
     bool ok = true;
     if (works) {
       for (int j = 0; j < mine; ++j) {
-        const int t = pair ? 2 * j + i : j;
+        const int q = j * streams + i, t = tile_of(q), buf = q % kBufs;
+        const uint32_t t_s = lanes + 128 * buf;
         uint32_t word[4] = {kFull, kFull, kFull, kFull};
         bool cut = false;
         if (masked) {
@@ -418,7 +455,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           for (int x = 0; x < 4; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
           cut = true;
         }
-        ok = warp_wait(s_full(i), j & 1, bail);
+        ok = warp_wait(s_full(buf), (q / kBufs) & 1, bail);
         if (!ok) break;
         tc_fence_after();
         float s[128];
@@ -432,15 +469,23 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int x = 4; x < 128; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
-        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c;
+        for (int x = 4; x < 124; x += 8) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) top[y] = max3(top[y], s[x + 2 * y], s[x + 2 * y + 1]);
+        }
+        const float mt = max3(max3(top[0], top[1], top[2]), max3(top[3], s[124], s[125]), fmaxf(s[126], s[127])) * a.c;
         const bool raise = mt > m + 8.0f;
         if (__any_sync(kFull, raise)) {
           const float back = raise ? (m == -INFINITY ? 0.0f : exp2_fast(m - mt)) : 1.0f;
           if (raise) m = mt;
           sum *= back;
-          // the output so far is complete: its last instruction came before the one that S waited for
+          // the output so far has to be complete.  A barrier tells only its last phase from the one before, so the product
+          // before the last one has to be known as done: with two streams it came before these scores, with one it is waited for.
           if (j > 0) {
+            if (streams == 1 && j > 1) ok = warp_wait(o_step(i), j & 1, bail);
+            ok = ok && warp_wait(o_step(i), (j - 1) & 1, bail);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < d16; x += 32) {
               float o[32];
@@ -454,22 +499,39 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         }
         const float off = m == -INFINITY ? 0.0f : -m;
         float2 part[4] = {};
-        uint32_t packed[64];
+        // in runs of eight pairs, so that the long chains of the pairs on the multiply-add pipe fill the gaps of the others
 #pragma unroll
-        for (int x = 0; x < 64; ++x) {
-          const float2 e = fma2(make_float2(s[2 * x], s[2 * x + 1]), make_float2(a.c, a.c), make_float2(off, off));
-          const float2 pr = exp2_pair<FBEV_POLY_FWD>(e, x);
-          part[x & 3] = add2(part[x & 3], pr);
-          packed[x] = pack2<T>(pr.x, pr.y);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            float2 e[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const int z = 64 * half + 2 * (x + y);
+              e[y] = fma2(make_float2(s[z], s[z + 1]), make_float2(a.c, a.c), make_float2(off, off));
+            }
+            exp2_run<FBEV_POLY_FWD>(e);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              part[y & 3] = add2(part[y & 3], e[y]);
+              packed[x + y] = pack2<T>(e[y].x, e[y].y);
+            }
+          }
+          tmem_st32(t_s + 32 * half, packed);
+          if (half == 0) {  // the tensor cores may begin
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_half(buf));
+          }
         }
-        tmem_st32(t_s, packed);
-        tmem_st32(t_s + 32, packed + 32);
         const float2 all = add2(add2(part[0], part[1]), add2(part[2], part[3]));
         sum += all.x + all.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(i));
+        if (lane == 0) mbar_arrive(p_full(buf));
       }
       if (ok && mine > 0) ok = warp_wait(o_full(i), 0, bail);
       // the second group is about to write over the ring: the first group's tiles must have been consumed too
@@ -552,7 +614,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<512>(s_tmem);
   }
 }
 

@@ -15,6 +15,11 @@ namespace fbev {
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// A value that is the same in all lanes, told so to the compiler: what the roles' loops are bounded and addressed by stays in
+// uniform registers.  Loops that look as if lanes could part would have every matrix instruction go through a search for
+// the lanes that issue it (measured: 1700 clocks for the dozen instructions of a step, longer than the step itself).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(kFull, v, 0); }
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -218,6 +223,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
