@@ -141,125 +141,104 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       const auto load_keys = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int tile) {
         for (int x = 0; x < NSUB; ++x) tma_load_4d(dst + x * kTileBytes, map, bar, 64 * x, g, tile * 128, b);
       };
-      const bool leader = elect_one();
-      if (leader) {
-        mbar_expect(x_full, 2 * x_bytes);
-        if (KV) {
-          load_keys(s_x, &a.x0, x_full, xt);
-          load_keys(s_x + kStageBytes, &a.x1, x_full, xt);
-        } else {
-          load_rows(s_x, &a.x0, x_full, xt, qb);
-          load_rows(s_x + kStageBytes, &a.x1, x_full, xt, b);
-        }
+      mbar_expect(x_full, 2 * x_bytes);
+      if (KV) {
+        load_keys(s_x, &a.x0, x_full, xt);
+        load_keys(s_x + kStageBytes, &a.x1, x_full, xt);
+      } else {
+        load_rows(s_x, &a.x0, x_full, xt, qb);
+        load_rows(s_x + kStageBytes, &a.x1, x_full, xt, b);
       }
       int slot = 0;
-      bool ok = true;
       const auto load = [&](const CUtensorMap* map, int t, int batch) {
         const int s = slot % kStages;
-        if (ok && slot >= kStages) ok = warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
-        if (!ok) return;
-        if (leader) {
-          mbar_expect(full(s), y_bytes);
-          if (KV)
-            load_rows(s_ring + s * kStageBytes, map, full(s), t0 + t, batch);
-          else
-            load_keys(s_ring + s * kStageBytes, map, full(s), t0 + t);
-        }
-        __syncwarp();
+        if (slot >= kStages) warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
+        mbar_expect(full(s), y_bytes);
+        if (KV)
+          load_rows(s_ring + s * kStageBytes, map, full(s), t0 + t, batch);
+        else
+          load_keys(s_ring + s * kStageBytes, map, full(s), t0 + t);
         ++slot;
       };
-      for (int t = 0; t < n && ok; ++t) {
+      for (int t = 0; t < n; ++t) {
         load(&a.y0, t, qb);
         load(&a.y1, t, b);
       }
-      if (!ok) {
+      if (__any_sync(kFull, *bail.flag != 0)) {
         // nothing may be left in flight when the block ends
         mbar_drain(x_full, 0);
         for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) mbar_drain(full(i % kStages), (i / kStages) & 1);
       }
     } else if (warp == 9 && n > 0) {
-      const bool leader = elect_one();
       // ---- matrix instructions -----------------------------------------------------------------------------------
       const int ksteps = (a.p.D + 15) / 16;
       const uint32_t i_s = umma_instr<T>(128, false, a.p.scale < 0.0f), i_dp = umma_instr<T>(128, false, false),
                      i_acc = umma_instr<T>(ksteps * 16, true, false);
       uint32_t fix_parity = 0;
-      bool ok = warp_wait(x_full, 0, bail);
-      const auto commit = [&](uint32_t bar) {
-        if (leader) umma_commit(bar);
-        __syncwarp();
-      };
+      warp_wait(x_full, 0, bail);
       const auto stage = [&](int slot) { return s_ring + (slot % kStages) * kStageBytes; };
-      const auto wait_full = [&](int slot) { ok = ok && warp_wait(full(slot % kStages), (slot / kStages) & 1, bail); };
+      const auto wait_full = [&](int slot) { warp_wait(full(slot % kStages), (slot / kStages) & 1, bail); };
       const auto product = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t instr) {  // X Y^T over the head's width
-        if (leader) {
 #pragma unroll
-          for (int i = 0; i < NSUB; ++i) {
-            const uint64_t da = desc_k_major(x + i * kTileBytes), db = desc_k_major(y + i * kTileBytes);
+        for (int i = 0; i < NSUB; ++i) {
+          const uint64_t da = desc_k_major(x + i * kTileBytes), db = desc_k_major(y + i * kTileBytes);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (i * 4 + k < ksteps) umma_ss(d, da + 2 * k, db + 2 * k, instr, i + k > 0);
-          }
+          for (int k = 0; k < 4; ++k)
+            if (i * 4 + k < ksteps) umma_ss(d, da + 2 * k, db + 2 * k, instr, i + k > 0);
         }
-        __syncwarp();
       };
       const auto accumulate = [&](uint32_t d, uint32_t t, uint32_t y, bool first) {  // 16-bit tile in tensor memory times Y
-        if (leader) {
-          const uint64_t db = desc_mn_major(y);
+        const uint64_t db = desc_mn_major(y);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) umma_ts(d, t + (k < 4 ? 8 * k : 32 + 8 * k), db + 128 * k, i_acc, !first || k > 0);
-        }
-        __syncwarp();
+        for (int k = 0; k < 8; ++k) umma_ts(d, t + (k < 4 ? 8 * k : 32 + 8 * k), db + 128 * k, i_acc, !first || k > 0);
       };
       const auto scores = [&](int t) {
         wait_full(2 * t);
         if (needs_fix(t)) {
           const int s = (2 * t) % kStages;
-          ok = ok && warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
+          warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
           fix_parity ^= 1u << s;
         }
-        if (!ok) return;
         tc_fence_after();
         product(tmem, s_x, stage(2 * t), i_s);
-        commit(s_full);
+        umma_commit(s_full);
       };
       const auto dprobs = [&](int t) {
         wait_full(2 * t + 1);
-        if (!ok) return;
         tc_fence_after();
         product(tmem + 128, s_x + kStageBytes, stage(2 * t + 1), i_dp);
-        commit(dp_full);
-        if (!KV) commit(empty((2 * t + 1) % kStages));
+        umma_commit(dp_full);
+        if (!KV) umma_commit(empty((2 * t + 1) % kStages));
       };
       scores(0);
-      if (ok) dprobs(0);
-      for (int t = 0; t < n && ok; ++t) {
-        ok = warp_wait(p_done, t & 1, bail);
-        if (!ok) break;
+      dprobs(0);
+      for (int t = 0; t < n; ++t) {
+        warp_wait(p_done, t & 1, bail);
         if (KV) {
           tc_fence_after();
           accumulate(tmem + 384, tmem, stage(2 * t + 1), t == 0);
-          commit(empty((2 * t + 1) % kStages));
+          umma_commit(empty((2 * t + 1) % kStages));
         }
         if (t + 1 < n) scores(t + 1);
-        ok = ok && warp_wait(ds_done, t & 1, bail);
-        if (!ok) break;
+        warp_wait(ds_done, t & 1, bail);
         tc_fence_after();
         accumulate(tmem + 256, tmem + 128, stage(2 * t), t == 0);
-        commit(empty((2 * t) % kStages));
+        umma_commit(empty((2 * t) % kStages));
         if (t + 1 < n) dprobs(t + 1);
       }
-      commit(ok ? acc_full : drained);
-      if (!ok) mbar_drain(drained, 0);
+      umma_commit(acc_full);
+      if (__any_sync(kFull, *bail.flag != 0)) {
+        umma_commit(drained);
+        mbar_drain(drained, 0);
+      }
     } else if (fixes && warp == 10 && n > 0) {
       // ---- key mask, keys that may not be attended -----------------------------------------------------------------
       const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
-      bool ok = true;
       const auto release = [&](int s) {
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
       };
-      for (int t = 0; t < n && ok; ++t) {
+      for (int t = 0; t < n ; ++t) {
         uint32_t word[4] = {kFull, kFull, kFull, kFull};
         const bool fix = needs_fix(t);
         if (fix) {
@@ -271,15 +250,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         }
         if (masked) {
           const int m = t % kMaskRing;
-          if (t >= kMaskRing) ok = warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
-          if (!ok) break;
+          if (t >= kMaskRing) warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
           if (lane < 4) s_mask[m][lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
           __syncwarp();
           if (lane == 0) mbar_arrive(m_full(m));
         }
         const int s = (2 * t) % kStages, s1 = (2 * t + 1) % kStages;
-        ok = warp_wait(full(s), ((2 * t) / kStages) & 1, bail);
-        if (!ok) break;
+        warp_wait(full(s), ((2 * t) / kStages) & 1, bail);
         if (fix) {
           if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
             for (int r = lane >> 3; r < 128; r += 4) {
@@ -293,8 +270,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
           if (lane == 0) mbar_arrive(fixed(s));
         }
         release(s);
-        ok = warp_wait(full(s1), ((2 * t + 1) / kStages) & 1, bail);
-        if (!ok) break;
+        warp_wait(full(s1), ((2 * t + 1) / kStages) & 1, bail);
         release(s1);
       }
     } else if (KV && warp == 10 && n > 0) {
@@ -304,7 +280,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       for (int t = 0; t < n; ++t) {
         const int m = t % kMaskRing;
         const float4 l = nlse[32 * t + lane], d = ndelta[32 * t + lane];
-        if (t >= kMaskRing && !warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail)) break;
+        if (t >= kMaskRing) warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
         *reinterpret_cast<float4*>(&s_stat[m][0][4 * lane]) = l;
         *reinterpret_cast<float4*>(&s_stat[m][1][4 * lane]) = d;
         __syncwarp();
@@ -322,13 +298,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     const int key = xt * 128 + r;                                    // dK, dV
     const float nl = KV ? 0.0f : a.nlse[((long long)bg * pl.row_tiles + xt) * 128 + r];
     const float nd = KV ? 0.0f : a.ndelta[((long long)bg * pl.row_tiles + xt) * 128 + r];
-    bool ok = true;
     for (int t = 0; t < n; ++t) {
       const int mr = t % kMaskRing;
       uint32_t word[2] = {kFull, kFull};
       if (!KV && masked) {
-        ok = warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
-        if (!ok) break;
+        warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
         word[0] = s_mask[mr][2 * h];
         word[1] = s_mask[mr][2 * h + 1];
         __syncwarp();
@@ -339,9 +313,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         for (int x = 0; x < 2; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
       }
       const bool cut = (word[0] & word[1]) != kFull;
-      ok = warp_wait(s_full, t & 1, bail);
-      if (ok && KV) ok = warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
-      if (!ok) break;
+      warp_wait(s_full, t & 1, bail);
+      if (KV) warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
       tc_fence_after();
       float p[64];
       tmem_ld32(t_s, p);
@@ -380,8 +353,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(p_done);
       }
-      ok = warp_wait(dp_full, t & 1, bail);
-      if (!ok) break;
+      warp_wait(dp_full, t & 1, bail);
       tc_fence_after();
       uint32_t packed[32];
 #pragma unroll
@@ -417,7 +389,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         if (KV) mbar_arrive(m_empty(mr));
       }
     }
-    if (ok && n > 0) ok = warp_wait(acc_full, 0, bail);
+    if (n > 0) warp_wait(acc_full, 0, bail);
     tc_fence_after();
     // ---- output: dQ column chunks in turn, or dK by the first group and dV by the second --------------------------------
     const int d16 = (a.p.D + 15) / 16 * 16;

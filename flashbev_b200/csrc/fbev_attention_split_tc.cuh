@@ -114,18 +114,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
     set_registers_down<80>();
     if (warp == 8 && n > 0) {
       // ---- loads -------------------------------------------------------------------------------------------------
-      const bool leader = elect_one();
       int slot = 0;
-      bool ok = true;
       const auto load = [&](const CUtensorMap* map, int chunk, int tile) {
         const int s = slot % kSplitStages;
-        if (ok && slot >= kSplitStages) ok = warp_wait(empty(s), ((slot / kSplitStages) - 1) & 1, bail);
-        if (!ok) return;
-        if (leader) {
-          mbar_expect(full(s), kSplitStageBytes);
-          tma_load_4d(s_ring + s * kSplitStageBytes, map, full(s), 64 * chunk, tile * 128, 0, bg);
-        }
-        __syncwarp();
+        if (slot >= kSplitStages) warp_wait(empty(s), ((slot / kSplitStages) - 1) & 1, bail);
+        mbar_expect(full(s), kSplitStageBytes);
+        tma_load_4d(s_ring + s * kSplitStageBytes, map, full(s), 64 * chunk, tile * 128, 0, bg);
         ++slot;
       };
       const auto load_scores = [&](int t) {
@@ -142,88 +136,74 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       };
       load_scores(0);
       if (kDs) load_dprobs(0);
-      for (int t = 0; t < n && ok; ++t) {
+      for (int t = 0; t < n ; ++t) {
         if (t + 1 < n) load_scores(t + 1);
         for (int c = 0; c < NC; ++c) load(&a.z, c, t0 + t);
         if (kDs && t + 1 < n) load_dprobs(t + 1);
       }
-      if (!ok)  // nothing may be left in flight when the block ends
+      if (__any_sync(kFull, *bail.flag != 0))  // nothing may be left in flight when the block ends
         for (int i = slot > kSplitStages ? slot - kSplitStages : 0; i < slot; ++i)
           mbar_drain(full(i % kSplitStages), (i / kSplitStages) & 1);
     } else if (warp == 9 && n > 0) {
       // ---- matrix instructions -----------------------------------------------------------------------------------
-      const bool leader = elect_one();
       const int ksteps = (a.p.D + 15) / 16;
       const uint32_t i_dp = umma_instr<__nv_bfloat16>(128, false, false);
       const uint32_t i_s = umma_instr<__nv_bfloat16>(128, false, a.p.scale < 0.0f);
       int slot = 0;
-      bool ok = true;
-      const auto commit = [&](uint32_t bar) {
-        if (leader) umma_commit(bar);
-        __syncwarp();
-      };
       const auto take = [&]() {
         const int s = slot % kSplitStages;
-        ok = ok && warp_wait(full(s), (slot / kSplitStages) & 1, bail);
+        warp_wait(full(s), (slot / kSplitStages) & 1, bail);
         ++slot;
         return s;
       };
       const auto product = [&](uint32_t d, uint32_t instr, uint32_t done) {  // X Y^T over the head's width
         for (int c = 0; c < NC; ++c) {
           const int sx = take(), sy = take();
-          if (!ok) return;
           tc_fence_after();
-          if (leader) {
-            const uint64_t dx = desc_k_major(s_ring + sx * kSplitStageBytes), dy = desc_k_major(s_ring + sy * kSplitStageBytes);
+          const uint64_t dx = desc_k_major(s_ring + sx * kSplitStageBytes), dy = desc_k_major(s_ring + sy * kSplitStageBytes);
 #pragma unroll
-            for (int i = 0; i < 6; ++i)
+          for (int i = 0; i < 6; ++i)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (c * 4 + k < ksteps)
-                  umma_ss(d, dx + split_x(i) * (kTileBytes / 16) + 2 * k, dy + split_y(i) * (kTileBytes / 16) + 2 * k, instr, c + i + k > 0);
-          }
-          __syncwarp();
-          commit(empty(sx));
-          commit(empty(sy));
+            for (int k = 0; k < 4; ++k)
+              if (c * 4 + k < ksteps)
+                umma_ss(d, dx + split_x(i) * (kTileBytes / 16) + 2 * k, dy + split_y(i) * (kTileBytes / 16) + 2 * k, instr, c + i + k > 0);
+          umma_commit(empty(sx));
+          umma_commit(empty(sy));
         }
-        commit(done);
+        umma_commit(done);
       };
       const auto accumulate = [&]() {  // the parts in tensor memory times Z, from zero
         for (int c = 0; c < NC; ++c) {
           const int s = take();
-          if (!ok) return;
           tc_fence_after();
           const int wide = ksteps * 16 - 64 * c;  // the last chunk may be narrow
           const uint32_t instr = umma_instr<__nv_bfloat16>(wide < 64 ? wide : 64, true, false);
-          if (leader && wide > 0) {
-            const uint64_t dz = desc_mn_major(s_ring + s * kSplitStageBytes);
+          const uint64_t dz = desc_mn_major(s_ring + s * kSplitStageBytes);
 #pragma unroll
-            for (int i = 0; i < 6; ++i)
+          for (int i = 0; i < 6; ++i)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const uint32_t half = k < 4 ? 0 : 1, at = 8 * (k & 3);
-                const uint32_t px = split_x(i) == 2 ? tmem + 256 + 32 * half + at : tmem + 128 + 64 * half + 32 * split_x(i) + at;
-                umma_ts(tmem + 320 + 64 * c, px, dz + split_y(i) * (kTileBytes / 16) + 128 * k, instr, i + k > 0);
-              }
-          }
-          __syncwarp();
-          commit(empty(s));
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t half = k < 4 ? 0 : 1, at = 8 * (k & 3);
+              const uint32_t px = split_x(i) == 2 ? tmem + 256 + 32 * half + at : tmem + 128 + 64 * half + 32 * split_x(i) + at;
+              umma_ts(tmem + 320 + 64 * c, px, dz + split_y(i) * (kTileBytes / 16) + 128 * k, instr, i + k > 0);
+            }
+          umma_commit(empty(s));
         }
-        commit(r_full);
+        umma_commit(r_full);
       };
       product(tmem, i_s, s_full);
-      if (kDs && ok) product(tmem + 128, i_dp, dp_full);
-      for (int t = 0; t < n && ok; ++t) {
+      if (kDs) product(tmem + 128, i_dp, dp_full);
+      for (int t = 0; t < n ; ++t) {
         if (t + 1 < n) {
-          ok = warp_wait(s_free, t & 1, bail);
-          if (ok) product(tmem, i_s, s_full);
+          warp_wait(s_free, t & 1, bail);
+          product(tmem, i_s, s_full);
         }
-        ok = ok && warp_wait(p_full, t & 1, bail);
-        if (ok) accumulate();
-        if (kDs && t + 1 < n && ok) product(tmem + 128, i_dp, dp_full);
+        warp_wait(p_full, t & 1, bail);
+        accumulate();
+        if (kDs && t + 1 < n) product(tmem + 128, i_dp, dp_full);
       }
-      if (!ok) {
-        commit(drained);
+      if (__any_sync(kFull, *bail.flag != 0)) {
+        umma_commit(drained);
         mbar_drain(drained, 0);
       }
     }
@@ -244,10 +224,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
 #pragma unroll
     for (int x = 0; x < W; ++x) acc[x] = 0.0f;
     float m = -INFINITY, sum = 0.0f;
-    bool ok = true;
     const auto absorb = [&](int t, float f) {  // the product of tile t, then the factor to the next maximum
-      ok = warp_wait(r_full, t & 1, bail);
-      if (!ok) return;
+      warp_wait(r_full, t & 1, bail);
       tc_fence_after();
 #pragma unroll
       for (int x = 0; x < W; x += 32) {
@@ -259,8 +237,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       }
     };
     for (int t = 0; t < n; ++t) {
-      ok = warp_wait(s_full, t & 1, bail);
-      if (!ok) break;
+      warp_wait(s_full, t & 1, bail);
       tc_fence_after();
       float p[64];
       tmem_ld32(lanes + 64 * h, p);
@@ -285,8 +262,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
         s_max[t & 1][h][r] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(top_full);
-        ok = warp_wait(top_full, t & 1, bail);
-        if (!ok) break;
+        warp_wait(top_full, t & 1, bail);
         const float mn = fmaxf(m, fmaxf(top, s_max[t & 1][h ^ 1][r]));
         back = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
         m = mn;
@@ -301,8 +277,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       }
       sum += (some[0] + some[1]) + (some[2] + some[3]);
       if (kDs) {
-        ok = warp_wait(dp_full, t & 1, bail);
-        if (!ok) break;
+        warp_wait(dp_full, t & 1, bail);
         tc_fence_after();
 #pragma unroll
         for (int y = 0; y < 64; y += 32) {
@@ -322,7 +297,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       }
       if (t > 0) {
         absorb(t - 1, back);
-        if (!ok) break;
       }
       // three parts; what is left after each is exact
 #pragma unroll
@@ -341,7 +315,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
     }
-    if (ok && n > 0) absorb(n - 1, 1.0f);
+    if (n > 0) absorb(n - 1, 1.0f);
     // ---- output --------------------------------------------------------------------------------------------------------
     float f = kDs ? a.p.scale : 1.0f;
     if (MODE == kSplitOut) {

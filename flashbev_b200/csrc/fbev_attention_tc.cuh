@@ -231,100 +231,80 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
     set_registers_down<80>();
     if (warp == 8 && n > 0) {
       // ---- loads -------------------------------------------------------------------------------------------------
-      const bool leader = elect_one();
-      if (leader) {
-        mbar_expect(q_full, (uint32_t)(tiles * NSUB * tile_rows * 128));
-        for (int i = 0; i < tiles; ++i)
-          for (int x = 0; x < NSUB; ++x)
-            tma_load_5d(s_q + i * kStageBytes + x * kTileBytes, &a.q, q_full, 64 * x, 0, g, (2 * rb + i) * pl.TL, a.p.q_shared ? 0 : b);
-      }
+      mbar_expect(q_full, (uint32_t)(tiles * NSUB * tile_rows * 128));
+      for (int i = 0; i < tiles; ++i)
+        for (int x = 0; x < NSUB; ++x)
+          tma_load_5d(s_q + i * kStageBytes + x * kTileBytes, &a.q, q_full, 64 * x, 0, g, (2 * rb + i) * pl.TL, a.p.q_shared ? 0 : b);
       int slot = 0;
-      bool ok = true;
       const auto load = [&](const CUtensorMap* map, int t) {
         const int s = slot % kStages;
-        if (ok && slot >= kStages) ok = warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
-        if (!ok) return;
-        if (leader) {
-          mbar_expect(full(s), kStageBytes);
-          for (int x = 0; x < NSUB; ++x)
-            tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, (t0 + t) * 128, b);
-        }
-        __syncwarp();
+        if (slot >= kStages) warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
+        mbar_expect(full(s), kStageBytes);
+        for (int x = 0; x < NSUB; ++x)
+          tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, (t0 + t) * 128, b);
         ++slot;
       };
       for (int q = 0; q < kBufs && q < steps; ++q)
         if (new_tile(q)) load(&a.k, tile_of(q));
-      for (int q = 0; q < steps && ok; ++q) {
+      for (int q = 0; q < steps; ++q) {
         if (new_tile(q)) load(&a.v, tile_of(q));
         if (q + kBufs < steps && new_tile(q + kBufs)) load(&a.k, tile_of(q + kBufs));
       }
-      if (!ok) {
+      if (__any_sync(kFull, *bail.flag != 0)) {
         // nothing may be left in flight when the block ends
         mbar_drain(q_full, 0);
         for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) mbar_drain(full(i % kStages), (i / kStages) & 1);
       }
     } else if (warp == 9 && n > 0) {
-      const bool leader = elect_one();
       // ---- matrix instructions -----------------------------------------------------------------------------------
       const bool negative = a.p.scale < 0.0f;
       const int ksteps = (a.p.D + 15) / 16;
       const uint32_t i_s = umma_instr<T>(128, false, negative), i_o = umma_instr<T>(ksteps * 16, true, false);
       uint32_t fix_parity = 0;
       int slot = 0;
-      bool ok = warp_wait(q_full, 0, bail);
-      const auto take = [&]() {  // next tile of the ring, as shared-memory address
+      warp_wait(q_full, 0, bail);
+      const auto take = [&]() {  // next tile of the ring
         const int s = slot % kStages;
-        ok = ok && warp_wait(full(s), (slot / kStages) & 1, bail);
+        warp_wait(full(s), (slot / kStages) & 1, bail);
         ++slot;
         return s;
       };
-      const auto commit = [&](uint32_t bar) {
-        if (leader) umma_commit(bar);
-        __syncwarp();
-      };
       const auto scores = [&](int q, int s) {
         tc_fence_after();
-        if (leader) {
-          const uint32_t d = tmem + 128 * (q % kBufs);
+        const uint32_t d = tmem + 128 * (q % kBufs);
 #pragma unroll
-          for (int x = 0; x < NSUB; ++x) {
-            const uint64_t da = desc_k_major(s_q + (pair ? 0 : stream_of(q)) * kStageBytes + x * kTileBytes);
-            const uint64_t db = desc_k_major(s_ring + s * kStageBytes + x * kTileBytes);
+        for (int x = 0; x < NSUB; ++x) {
+          const uint64_t da = desc_k_major(s_q + (pair ? 0 : stream_of(q)) * kStageBytes + x * kTileBytes);
+          const uint64_t db = desc_k_major(s_ring + s * kStageBytes + x * kTileBytes);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (x * 4 + k < ksteps) umma_ss(d, da + 2 * k, db + 2 * k, i_s, x + k > 0);
-          }
-          umma_commit(s_full(q % kBufs));
+          for (int k = 0; k < 4; ++k)
+            if (x * 4 + k < ksteps) umma_ss(d, da + 2 * k, db + 2 * k, i_s, x + k > 0);
         }
-        __syncwarp();
+        umma_commit(s_full(q % kBufs));
       };
       const auto values = [&](int q, int s, int half, bool first) {  // half of the keys
         tc_fence_after();
-        if (leader) {
-          const uint64_t db = desc_mn_major(s_ring + s * kStageBytes);
-          const uint32_t d = tmem + Shape::kOutAt + Shape::kOutCols * stream_of(q), p = tmem + 128 * (q % kBufs);
+        const uint64_t db = desc_mn_major(s_ring + s * kStageBytes);
+        const uint32_t d = tmem + Shape::kOutAt + Shape::kOutCols * stream_of(q), p = tmem + 128 * (q % kBufs);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int kk = 4 * half + k;
-            umma_ts(d, p + 8 * kk, db + 128 * kk, i_o, !first || kk > 0);
-          }
+        for (int k = 0; k < 4; ++k) {
+          const int kk = 4 * half + k;
+          umma_ts(d, p + 8 * kk, db + 128 * kk, i_o, !first || kk > 0);
         }
-        __syncwarp();
       };
       const auto fix_wait = [&](int t, int s) {
         if (!needs_fix(t)) return;
-        ok = ok && warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
+        warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
         fix_parity ^= 1u << s;
       };
       int sk = 0, sv = 0;
       const auto last_use = [&](int q) { return pair || streams == 1 || (q & 1) == 1; };  // of the tile of keys or values
-      for (int q = 0; q < kBufs && q < steps && ok; ++q) {
+      for (int q = 0; q < kBufs && q < steps; ++q) {
         if (new_tile(q)) sk = take();
-        if (!ok) break;
         scores(q, sk);
-        if (last_use(q)) commit(empty(sk));
+        if (last_use(q)) umma_commit(empty(sk));
       }
-      for (int q = 0; q < steps && ok; ++q) {
+      for (int q = 0; q < steps; ++q) {
         const int i = stream_of(q), buf = q % kBufs, parity = (q / kBufs) & 1;
         if (new_tile(q)) {
           sv = take();
@@ -332,33 +312,29 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         }
         const bool more = q + kBufs < steps;
         if (more && new_tile(q + kBufs)) sk = take();
-        ok = ok && warp_wait(p_half(buf), parity, bail);
-        if (!ok) break;
+        warp_wait(p_half(buf), parity, bail);
         values(q, sv, 0, q < streams);
-        ok = warp_wait(p_full(buf), parity, bail);
-        if (!ok) break;
+        warp_wait(p_full(buf), parity, bail);
         values(q, sv, 1, false);
-        if (more) scores(q + kBufs, sk);
-        if (leader) {
-          umma_commit(o_step(i));
-          if (q + streams >= steps) umma_commit(o_full(i));
-          if (last_use(q)) umma_commit(empty(sv));
-          if (more && last_use(q + kBufs)) umma_commit(empty(sk));
+        umma_commit(o_step(i));
+        if (q + streams >= steps) umma_commit(o_full(i));
+        if (last_use(q)) umma_commit(empty(sv));
+        if (more) {
+          scores(q + kBufs, sk);
+          if (last_use(q + kBufs)) umma_commit(empty(sk));
         }
-        __syncwarp();
       }
-      if (!ok) {
-        commit(drained);
+      if (__any_sync(kFull, *bail.flag != 0)) {
+        umma_commit(drained);
         mbar_drain(drained, 0);
       }
     } else if (warp == 10 && n > 0 && fixes) {
       // ---- key mask, values that may not be attended ---------------------------------------------------------------
       const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
-      bool ok = true;
       int slot = 0;
       const auto follow = [&]() {  // the next stage of the ring, once it is loaded
         const int s = slot % kStages;
-        ok = ok && warp_wait(full(s), (slot / kStages) & 1, bail);
+        warp_wait(full(s), (slot / kStages) & 1, bail);
         ++slot;
         return s;
       };
@@ -368,12 +344,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       };
       for (int q = 0; q < kBufs && q < steps; ++q)
         if (new_tile(q)) release(follow());
-      for (int q = 0; q < steps && ok; ++q) {
+      for (int q = 0; q < steps ; ++q) {
         const bool keys_next = q + kBufs < steps && new_tile(q + kBufs);
         if (!new_tile(q)) {
           if (keys_next) {
             const int sk = follow();
-            if (!ok) break;
             release(sk);
           }
           continue;
@@ -390,14 +365,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         }
         if (masked) {
           const int m = t % kMaskRing;
-          if (t >= kMaskRing) ok = warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
-          if (!ok) break;
+          if (t >= kMaskRing) warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
           if (lane < 4) s_mask[m][lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
           __syncwarp();
           if (lane == 0) mbar_arrive(m_full(m));
         }
         const int s = follow();
-        if (!ok) break;
         if (fix) {
           if ((word[0] & word[1] & word[2] & word[3]) != kFull) {
             // a row's 128 bytes: eight lanes, four rows at a time (the swizzle permutes within the row, zeros do not care)
@@ -414,7 +387,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         release(s);
         if (keys_next) {
           const int sk = follow();
-          if (!ok) break;
           release(sk);
         }
       }
@@ -433,7 +405,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
     const bool live = works && r < tile_rows && row < rows;
     const int d16 = (a.p.D + 15) / 16 * 16;
     float m = -INFINITY, sum = 0.0f;
-    bool ok = true;
     if (works) {
       for (int j = 0; j < mine; ++j) {
         const int q = j * streams + i, t = tile_of(q), buf = q % kBufs;
@@ -442,8 +413,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         bool cut = false;
         if (masked) {
           const int mr = t % kMaskRing;
-          ok = warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
-          if (!ok) break;
+          warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
 #pragma unroll
           for (int x = 0; x < 4; ++x) word[x] = s_mask[mr][x];
           __syncwarp();
@@ -455,8 +425,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           for (int x = 0; x < 4; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
           cut = true;
         }
-        ok = warp_wait(s_full(buf), (q / kBufs) & 1, bail);
-        if (!ok) break;
+        warp_wait(s_full(buf), (q / kBufs) & 1, bail);
         tc_fence_after();
         float s[128];
 #pragma unroll
@@ -482,9 +451,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           // the output so far has to be complete.  A barrier tells only its last phase from the one before, so the product
           // before the last one has to be known as done: with two streams it came before these scores, with one it is waited for.
           if (j > 0) {
-            if (streams == 1 && j > 1) ok = warp_wait(o_step(i), j & 1, bail);
-            ok = ok && warp_wait(o_step(i), (j - 1) & 1, bail);
-            if (!ok) break;
+            if (streams == 1 && j > 1) warp_wait(o_step(i), j & 1, bail);
+            warp_wait(o_step(i), (j - 1) & 1, bail);
             tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < d16; x += 32) {
@@ -533,9 +501,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(buf));
       }
-      if (ok && mine > 0) ok = warp_wait(o_full(i), 0, bail);
+      if (mine > 0) warp_wait(o_full(i), 0, bail);
       // the second group is about to write over the ring: the first group's tiles must have been consumed too
-      if (ok && pair && i == 1 && mine > 0) ok = warp_wait(o_full(0), 0, bail);
+      if (pair && i == 1 && mine > 0) warp_wait(o_full(0), 0, bail);
       __syncwarp();
       tc_fence_after();
     }

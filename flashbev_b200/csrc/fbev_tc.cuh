@@ -26,8 +26,9 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {  // by a whole warp
+  asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar), "r"(bytes)
+               : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -45,53 +46,50 @@ struct Bail {
   uint32_t* status;
 };
 
-// Waits until the phase of the given parity has completed.  Ends after about two seconds, or soon after another thread
-// of the block gave up: false, and every role then leaves its loop.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
-  if (mbar_try(bar, parity)) return true;
+// Waits until the phase of the given parity has completed.  Gives up after about two seconds, or soon after another thread
+// of the block did.  Nothing is returned: a block that gave up runs its loops to their end with whatever it has, all its
+// accesses being in bounds whatever the data, and the status word tells that the result is not valid.
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
+  if (mbar_try(bar, parity)) return;
   const long long t0 = clock64();
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 32; ++i)
-      if (mbar_try(bar, parity)) return true;
-    if (*bail.flag != 0) return false;
+      if (mbar_try(bar, parity)) return;
+    if (*bail.flag != 0) return;
     if (clock64() - t0 > 4000000000ll) {
       *bail.flag = 1;
       if (bail.status != nullptr) atomicOr(bail.status, (uint32_t)FBEV_DEV_TIMEOUT);
-      return false;
+      return;
     }
   }
 }
-
-// the same for a whole warp, which stays together
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
-  return __all_sync(kFull, mbar_wait(bar, parity, bail));
+// the same for a whole warp, which is together afterwards
+__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
+  mbar_wait(bar, parity, bail);
+  __syncwarp();
 }
-// for a while only, whatever became of the others: before a block ends early
+// for a while only, whatever became of the others: before a block that gave up ends
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
   const long long t0 = clock64();
   while (!mbar_try(bar, parity) && clock64() - t0 < 1000000000ll) {
   }
 }
 
-// One lane of a converged warp, the same each time.  Loads and matrix instructions are issued by it from loops that the
-// whole warp runs: their descriptors live in uniform registers, which a loop run by one lane alone would share with lanes
-// that are elsewhere.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t pred;
-  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(pred));
-  return pred != 0;
-}
-
+// Loads, matrix instructions and commits are called by whole warps and issued by one elected lane (the same each time), by
+// a predicate inside the instruction's own text: the loops around stay those of a warp, and their operands in uniform
+// registers.  A loop run by one lane alone would share those registers with lanes that are elsewhere.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n}" ::"r"(dst),
       "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w, int u) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n}" ::"r"(
           dst),
       "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
       : "memory");
@@ -172,18 +170,18 @@ __host__ __device__ constexpr uint32_t umma_instr(int n, bool b_mn_major, bool n
          (128u >> 4) << 24;
 }
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+  asm volatile("{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
                "l"(b), "r"(instr), "r"((uint32_t)accumulate)
                : "memory");
 }
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
+  asm volatile("{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
                "l"(b), "r"(instr), "r"((uint32_t)accumulate)
                : "memory");
 }
 // the barrier's phase gets one arrival when every matrix instruction this thread issued so far is done
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar) : "memory");
 }
 
 template <int N>
