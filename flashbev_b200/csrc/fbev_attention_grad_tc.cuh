@@ -445,33 +445,49 @@ __global__ void __launch_bounds__(256) att_sum_kernel(const float* __restrict__ 
   }
 }
 
-// -lse and -delta = -<out, grad_out> of every row of the padded row tiles: eight lanes a row, 16 bytes a load
+// -lse and -delta = -<out, grad_out> of every row of the padded row tiles: eight lanes share a row, 16 bytes a load, and have
+// kStatRows rows in flight
+constexpr int kStatRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ FbevAttention p, int TL, int row_tiles, const T* __restrict__ out,
                                                        const T* __restrict__ go, const float* __restrict__ lse, float* __restrict__ nlse,
                                                        float* __restrict__ ndelta) {
-  const long long rows = att_rows(p), at = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
   const int lane = threadIdx.x & 7, G = p.Hq / p.Hkv;
-  const long long tile = at >> 7, bg = tile / row_tiles;
-  const int r = (int)(at & 127);
-  const long long row = (tile - bg * row_tiles) * TL * G + r;
-  const bool there = bg < (long long)p.B * p.Hkv, live = there && r < TL * G && row < rows;
-  float d = 0.0f;
-  if (live) {
-    const long long b = bg / p.Hkv, g = bg - b * p.Hkv, l = row / G;
-    const long long head = ((b * p.Lq + l) * p.Hq + g * G + (row - l * G)) * p.D;
-    for (int c = lane * 8; c < p.D; c += 64) {
-      const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(out + head + c);
-      const Pack<T, 8> y = *reinterpret_cast<const Pack<T, 8>*>(go + head + c);
+  const unsigned rows = (unsigned)att_rows(p);
+  // blocks of 128 rows: one row tile
+  const unsigned bg = blockIdx.x / (unsigned)row_tiles, tile = blockIdx.x - bg * (unsigned)row_tiles, b = bg / p.Hkv, g = bg - b * p.Hkv;
+  float d[kStatRows], l[kStatRows];
+  Pack<T, 8> x[kStatRows][2], y[kStatRows][2];
+  bool live[kStatRows];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d = fmaf(to_float(x.v[e]), to_float(y.v[e]), d);
-    }
+  for (int k = 0; k < kStatRows; ++k) {
+    const unsigned r = 32 * k + (threadIdx.x >> 3), row = tile * TL * G + r, q = row / G;
+    live[k] = r < (unsigned)(TL * G) && row < rows;
+    const long long head = (((long long)b * p.Lq + q) * p.Hq + g * G + (row - q * G)) * p.D;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (live[k] && lane * 8 + 64 * i < p.D) {
+        x[k][i] = *reinterpret_cast<const Pack<T, 8>*>(out + head + lane * 8 + 64 * i);
+        y[k][i] = *reinterpret_cast<const Pack<T, 8>*>(go + head + lane * 8 + 64 * i);
+      }
+    l[k] = live[k] && lane == 0 ? lse[bg * att_rows_padded(p) + row] : INFINITY;
   }
 #pragma unroll
-  for (int s = 4; s > 0; s >>= 1) d += __shfl_xor_sync(kFull, d, s);
-  if (there && lane == 0) {
-    nlse[at] = live ? -lse[bg * att_rows_padded(p) + row] : -INFINITY;
-    ndelta[at] = -d;
+  for (int k = 0; k < kStatRows; ++k) {
+    d[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (live[k] && lane * 8 + 64 * i < p.D) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[k] = fmaf(to_float(x[k][i].v[e]), to_float(y[k][i].v[e]), d[k]);
+      }
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) d[k] += __shfl_xor_sync(kFull, d[k], s);
+    if (lane == 0) {
+      const long long at = (long long)blockIdx.x * 128 + 32 * k + (threadIdx.x >> 3);
+      nlse[at] = -l[k];
+      ndelta[at] = -d[k];
+    }
   }
   grid_dependency_trigger();
 }

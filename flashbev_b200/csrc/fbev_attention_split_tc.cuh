@@ -339,10 +339,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       const long long heads = (long long)a.p.B * a.p.Hkv;
       const long long at = kKeyRows ? (((long long)b * a.p.Lk + row) * a.p.Hkv + g) * a.p.D
                                     : (((long long)b * a.p.Lq + row / G) * a.p.Hq + g * G + row % G) * a.p.D;
-      // parts of out are laid out by row for the join, those of the gradients like the gradients
+      // parts of out are laid out by row tile for the join, those of the gradients like the gradients
       float* part = a.part;
       if (parted) {
-        if (MODE == kSplitOut) part += ((split * heads + bg) * a.x_rows + row) * a.p.D;
+        if (MODE == kSplitOut) part += ((split * heads + bg) * a.x_tiles * 128 + row) * a.p.D;
         else part += split * (kKeyRows ? (long long)a.p.B * a.p.Lk * a.p.Hkv : (long long)a.p.B * a.p.Lq * a.p.Hq) * a.p.D + at;
       }
       float* dst = a.g + at;
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       }
       if (MODE == kSplitOut && h == 0) {
         const long long padded = att_rows_padded(a.p);
-        if (parted) a.part_lse[(split * heads + bg) * padded + row] = sum == 0.0f ? -INFINITY : m + log2f(sum);
+        if (parted) a.part_lse[(split * heads + bg) * a.x_tiles * 128 + row] = sum == 0.0f ? -INFINITY : m + log2f(sum);
         else if (a.lse != nullptr) a.lse[bg * padded + row] = sum == 0.0f ? INFINITY : m + log2f(sum);
       }
     }

@@ -33,8 +33,10 @@ struct AttPlan {
   int G, TL;           // heads of a group, queries in a row tile (TL * G <= 128 rows)
   int row_tiles;       // of a (sample, key head)
   int pair;            // one row tile, even and odd key tiles
-  int row_blocks;      // blocks along the rows
-  int splits, per_split;  // blocks along the keys and their key tiles
+  int row_blocks;      // units along the rows: up to two row tiles each
+  // The first `whole` units (of all samples and key heads) are a block each; each of the others is split along the keys
+  // over `splits` blocks of `per_split` key tiles.
+  int whole, splits, per_split;
 };
 
 struct AttFwdArgs {
@@ -43,14 +45,16 @@ struct AttFwdArgs {
   AttPlan pl;
   void* out;
   float* lse;       // final statistics or null
-  float* part;      // [splits][B * Hkv][rows][D] with splits > 1
-  float* part_lse;  // [splits][B * Hkv][rows_padded]
+  float* part;      // [splits][split units][256 rows][D]
+  float* part_lse;  // [splits][split units][256 rows]
   float c;          // |scale| * log2 e
 };
 
 template <int NSUB>
 struct AttFwdShape {
   static constexpr int kBufs = NSUB == 1 ? 3 : 2;      // score tiles in tensor memory
+  // with two score tiles a group waits for P V and the next scores: P V then begins at half of P
+  static constexpr bool kHalves = kBufs == 2;
   static constexpr int kOutAt = 128 * kBufs, kOutCols = NSUB == 1 ? 64 : 128;
   static constexpr int kStages = NSUB == 1 ? 10 : 5;
   static constexpr uint32_t kStageBytes = NSUB * kTileBytes;
@@ -64,7 +68,7 @@ struct AttFwdShape {
 // -infinity leaves a weight that no sum notices, and rows without any key are told by their maximum.
 // this many of eight pairs
 #ifndef FBEV_POLY_FWD
-#define FBEV_POLY_FWD 3
+#define FBEV_POLY_FWD 1
 #endif
 #ifndef FBEV_POLY_GRAD
 #define FBEV_POLY_GRAD 3
@@ -149,15 +153,18 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   const AttPlan& pl = a.pl;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // block -> (split, row block, sample, key head); row blocks of one key head are neighbours and share its keys in L2
-  int u = blockIdx.x;
-  const int split = u % pl.splits;
-  u /= pl.splits;
+  int u = blockIdx.x, split = 0;
+  const bool parted = u >= pl.whole;
+  if (parted) {
+    split = (u - pl.whole) % pl.splits;
+    u = pl.whole + (u - pl.whole) / pl.splits;
+  }
   const int rb = u % pl.row_blocks;
   const int bg = u / pl.row_blocks, b = bg / a.p.Hkv, g = bg % a.p.Hkv;
   const int keys = uniform(att_keys(a.p, b));
   const int t0 = split * pl.per_split;
   int n = (keys + 127) / 128 - t0;  // key tiles of this block
-  n = n < 0 ? 0 : n > pl.per_split ? pl.per_split : n;
+  n = n < 0 ? 0 : parted && n > pl.per_split ? pl.per_split : n;
   const bool pair = pl.pair != 0;
   const int tiles = pair ? 1 : (pl.row_tiles - 2 * rb < 2 ? 1 : 2);  // row tiles of this block
   const bool masked = a.p.key_mask != nullptr;
@@ -312,9 +319,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         }
         const bool more = q + kBufs < steps;
         if (more && new_tile(q + kBufs)) sk = take();
-        warp_wait(p_half(buf), parity, bail);
-        values(q, sv, 0, q < streams);
+        if (Shape::kHalves) {
+          warp_wait(p_half(buf), parity, bail);
+          values(q, sv, 0, q < streams);
+        }
         warp_wait(p_full(buf), parity, bail);
+        if (!Shape::kHalves) values(q, sv, 0, q < streams);
         values(q, sv, 1, false);
         umma_commit(o_step(i));
         if (q + streams >= steps) umma_commit(o_full(i));
@@ -487,7 +497,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
             }
           }
           tmem_st32(t_s + 32 * half, packed);
-          if (half == 0) {  // the tensor cores may begin
+          if (half == 0 && Shape::kHalves) {  // the tensor cores may begin
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -538,11 +548,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       }
       const bool none = m == -INFINITY;  // no key
       const float inv = none ? 0.0f : 1.0f / sum;
-      const bool parted = pl.splits > 1;
       const long long l = row / pl.G;
       T* dst = reinterpret_cast<T*>(a.out) + (((long long)b * a.p.Lq + l) * a.p.Hq + g * pl.G + (int)(row - l * pl.G)) * a.p.D;
-      const long long at = (long long)split * a.p.B * a.p.Hkv + bg;
-      float* dpart = a.part + (at * rows + row) * a.p.D;
+      const long long units = (long long)a.p.B * a.p.Hkv * pl.row_blocks - pl.whole;
+      const long long at = (split * units + (u - pl.whole)) * 256 + (pair ? 0 : 128 * i) + r;
+      float* dpart = parted ? a.part + at * a.p.D : nullptr;
       const float* s_join = reinterpret_cast<const float*>(s_raw + (s_ring - smem_addr(s_raw)));
       __syncwarp();
       if (works) {
@@ -571,7 +581,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       }
       if (live) {
         if (parted)
-          a.part_lse[at * att_rows_padded(a.p) + row] = none ? -INFINITY : m + log2f(sum);
+          a.part_lse[at] = none ? -INFINITY : m + log2f(sum);
         else if (a.lse != nullptr)
           a.lse[(long long)bg * att_rows_padded(a.p) + row] = none ? INFINITY : m + log2f(sum);
       }
@@ -586,42 +596,58 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   }
 }
 
-// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s: a warp per row
+struct JoinArgs {
+  const float* part;      // [splits][units][slots][D]
+  const float* part_lse;  // [splits][units][slots]
+  float* lse;             // or null
+  int splits, slots;      // rows of a unit in the parts: 128 or 256
+  int whole, units;       // units before the first split one, split units
+  int per_head;           // units of a (sample, key head)
+  int tile_rows;          // rows of a row tile of 128
+};
+
+// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s: a block per row, its warps take the splits in
+// turn (in a fixed order) and add up in shared memory
 template <typename T>
-__global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ FbevAttention p, const float* __restrict__ part,
-                                                       const float* __restrict__ part_lse, int splits, T* __restrict__ out,
-                                                       float* __restrict__ lse) {
+__global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ FbevAttention p, const __grid_constant__ JoinArgs a, T* __restrict__ out) {
+  __shared__ float s_out[4][128], s_total[4];
   grid_dependency_wait();
-  const long long rows = att_rows(p), padded = att_rows_padded(p), heads = (long long)p.B * p.Hkv;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (unit >= rows * heads) return;
-  const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
-  const long long bg = unit / rows, row = unit - bg * rows;
-  const float* pl = part_lse + bg * padded + row;
+  const int u = blockIdx.x / a.slots, slot = blockIdx.x % a.slots;
+  const int unit = a.whole + u, bg = unit / a.per_head, G = p.Hq / p.Hkv;
+  const long long rows = att_rows(p);
+  const long long row = ((long long)(unit - bg * a.per_head) * (a.slots / 128) + slot / 128) * a.tile_rows + slot % 128;
+  if (slot % 128 >= a.tile_rows || row >= rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long step = (long long)a.units * a.slots, at = (long long)u * a.slots + slot;
   float top = -INFINITY;
-  for (int s = lane; s < splits; s += 32) top = fmaxf(top, pl[s * heads * padded]);
+  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_lse[s * step + at]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
   float total = 0.0f, o[4] = {};
   if (top != -INFINITY) {
-    for (int s = 0; s < splits; ++s) {
-      const float w = exp2_fast(pl[s * heads * padded] - top);
-      if (w == 0.0f) continue;
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += 4) {
+      const float w = exp2_fast(a.part_lse[s * step + at] - top);
+      const float* src = a.part + (s * step + at) * p.D;
       total += w;
-      const float* src = part + ((s * heads + bg) * rows + row) * p.D;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (lane + 32 * i < p.D) o[i] = fmaf(w, src[lane + 32 * i], o[i]);
     }
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const long long l = row / G;
-  const int b = (int)(bg / p.Hkv), h = (int)(bg % p.Hkv) * G + (int)(row - l * G);
-  T* dst = out + (((long long)b * p.Lq + l) * p.Hq + h) * p.D;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < p.D) dst[lane + 32 * i] = from_float<T>(o[i] * inv);
-  if (lse != nullptr && lane == 0) lse[bg * padded + row] = total == 0.0f ? INFINITY : top + log2f(total);
+  for (int i = 0; i < 4; ++i) s_out[warp][lane + 32 * i] = o[i];
+  if (lane == 0) s_total[warp] = total;
+  __syncthreads();
+  total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+  const int c = threadIdx.x;
+  const long long l = row / G;
+  const int b = bg / p.Hkv, h = (bg % p.Hkv) * G + (int)(row - l * G);
+  if (c < p.D) {
+    const float v = (s_out[0][c] + s_out[1][c]) + (s_out[2][c] + s_out[3][c]);
+    out[(((long long)b * p.Lq + l) * p.Hq + h) * p.D + c] = from_float<T>(total == 0.0f ? 0.0f : v / total);
+  }
+  if (a.lse != nullptr && c == 0) a.lse[bg * att_rows_padded(p) + row] = total == 0.0f ? INFINITY : top + log2f(total);
 }
 
 }  // namespace fbev

@@ -28,7 +28,7 @@ static int check_attention(const FbevAttention* p) {
   if (p->B < 0 || p->Lq < 0 || p->Lk < 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->D <= 0 || p->D > 128)
     return FBEV_ERR_SHAPE;
   if (att_rows(*p) >= (1ll << 31) || (long long)p->B * p->Hq >= (1ll << 31)) return FBEV_ERR_RANGE;
-  if ((long long)p->B * p->Hkv * (att_rows(*p) / 4 + 1) >= (1ll << 31) || (long long)p->B * p->Hkv * (p->Lk / 4 + 1) >= (1ll << 31))
+  if ((long long)p->B * p->Hkv * (att_rows(*p) + 256) >= (1ll << 31) || (long long)p->B * p->Hkv * (p->Lk + 256ll) >= (1ll << 31))
     return FBEV_ERR_RANGE;  // blocks of a launch
   if ((uintptr_t)p->key_lengths % 4 || (uintptr_t)p->status % 4) return FBEV_ERR_ALIGN;
   const size_t es = size_of(p->dtype);
@@ -63,6 +63,46 @@ static bool direct(const FbevAttention& p) {
          tma_operand(p.k, p.k_stride, {p.B, p.Lk, p.Hkv}, false) && tma_operand(p.v, p.v_stride, {p.B, p.Lk, p.Hkv}, false);
 }
 
+// How units of work (a block each, `tiles` steps long) are spread over the SMs.  Blocks of one length run in waves of one per
+// SM, so the last wave may leave most of them idle; a unit that is split along its steps runs as several shorter blocks,
+// whose parts have to be written and summed.  The choice is the shortest of: nothing split; all units split into s; where
+// `tail` is set, the units of the last wave alone split into s.  Times are in steps, 3 for a block's begin and end and
+// `part` for the parts of a unit (writing and reading, spread over all SMs); where the samples' lengths differ the mean over
+// full, three quarter and half length counts, since all blocks of a short sample end early.  Only full waves are left whole
+// by a split tail.
+struct SplitChoice {
+  int whole, splits, per_split;
+};
+static SplitChoice choose_splits(int units, int tiles, double part, bool ragged, bool tail) {
+  const auto waves = [&](double blocks) { return (double)((long long)((blocks + kSms - 1) / kSms)); };
+  const auto all = [&](int s, int per) {
+    if (!ragged) return waves((double)units * s) * (per + 3);
+    double t = 0;
+    for (const double f : {1.0, 0.75, 0.5}) t += waves((long long)(f * units * s)) * (per + 3) / 3;
+    return t;
+  };
+  SplitChoice best{units, 1, tiles > 0 ? tiles : 1};
+  double cost = all(1, tiles);
+  const int full = units / kSms * kSms, rest = units - full;
+  for (int want = 2; want <= tiles && want <= 128; ++want) {
+    const int per = (tiles + want - 1) / want, s = (tiles + per - 1) / per;
+    if (s != want) continue;
+    const double c = all(s, per) + (units * s / (double)kSms) * part + 2;
+    if (c < 0.98 * cost) {
+      cost = c;
+      best = {0, s, per};
+    }
+    if (tail && full > 0 && rest > 0) {
+      const double d = full / kSms * (tiles + 3) + waves((double)rest * s) * (per + 3) + (rest * s / (double)kSms) * part + 2;
+      if (d < 0.98 * cost) {
+        cost = d;
+        best = {full, s, per};
+      }
+    }
+  }
+  return best;
+}
+
 static AttPlan attention_plan(const FbevAttention& p) {
   AttPlan pl{};
   pl.G = p.Hq / p.Hkv;
@@ -70,18 +110,16 @@ static AttPlan attention_plan(const FbevAttention& p) {
   pl.row_tiles = (p.Lq + pl.TL - 1) / pl.TL;
   pl.pair = pl.row_tiles == 1;
   pl.row_blocks = (pl.row_tiles + 1) / 2;
-  // split the keys when the blocks along rows, heads and samples leave SMs idle
-  const long long blocks = (long long)p.B * p.Hkv * pl.row_blocks;
-  const int key_tiles = (p.Lk + 127) / 128;
-  long long splits = blocks < kSms ? kSms / blocks : 1;
-  if (splits > key_tiles) splits = key_tiles;
-  pl.per_split = (int)((key_tiles + splits - 1) / splits);
-  pl.splits = (key_tiles + pl.per_split - 1) / pl.per_split;
+  const int units = p.B * p.Hkv * pl.row_blocks, key_tiles = (p.Lk + 127) / 128;
+  const SplitChoice c = choose_splits(units, key_tiles, 0.5 * pl.G * pl.TL * 2 * p.D * 4 / 40000.0, p.key_lengths != nullptr, true);
+  pl.whole = c.whole;
+  pl.splits = c.splits;
+  pl.per_split = c.per_split;
   return pl;
 }
 
 static size_t split_output_bytes(const FbevAttention& p, const AttPlan& pl) {
-  return round_up((size_t)pl.splits * p.B * p.Hkv * att_rows(p) * p.D * 4, 256);
+  return round_up((size_t)pl.splits * (p.B * p.Hkv * pl.row_blocks - pl.whole) * 256 * p.D * 4, 256);
 }
 // ---- three-part operands ----------------------------------------------------------------------------------------------
 
@@ -95,13 +133,10 @@ static SplitPlan split_plan(const FbevAttention& p, int mode) {
   pl.x_tiles = key_rows ? key_tiles : row_tiles;
   pl.y_tiles = key_rows ? row_tiles : key_tiles;
   pl.x_rows = key_rows ? p.Lk : (int)att_rows(p);
-  const long long blocks = (long long)p.B * p.Hkv * pl.x_tiles;
-  long long splits = blocks > 0 && blocks < kSms ? kSms / blocks : 1;
-  if (splits > pl.y_tiles) splits = pl.y_tiles > 0 ? pl.y_tiles : 1;
-  pl.per_split = (int)((pl.y_tiles + splits - 1) / splits);
-  if (pl.per_split < 1) pl.per_split = 1;
-  pl.splits = (pl.y_tiles + pl.per_split - 1) / pl.per_split;
-  if (pl.splits < 1) pl.splits = 1;
+  // a step takes about four times as long as one of the 16-bit kernels
+  const SplitChoice c = choose_splits(p.B * p.Hkv * pl.x_tiles, pl.y_tiles, 128.0 * p.D * 4 / 160000.0, p.key_lengths != nullptr, false);
+  pl.splits = c.splits;
+  pl.per_split = c.per_split;
   return pl;
 }
 
@@ -135,11 +170,11 @@ static SplitLayout split_layout(const FbevAttention& p, bool backward) {
   for (int mode = backward ? kSplitDv : kSplitOut; mode <= (backward ? kSplitDk : kSplitOut); ++mode) {
     const SplitPlan pl = split_plan(p, mode);
     if (pl.splits == 1 && p.dtype == FBEV_F32) continue;
-    const size_t n = (size_t)pl.splits * (mode == kSplitDv || mode == kSplitDk ? keys : rows) * p.D * 4;
+    const size_t n = (size_t)pl.splits * (mode == kSplitDv || mode == kSplitDk ? keys : mode == kSplitDq ? rows : heads * pl.x_tiles * 128) * p.D * 4;
     if (n > part) part = n;
   }
   l.part = take(round_up(part, 256));
-  if (!backward && part > 0) l.part_lse = take(round_up((size_t)split_plan(p, kSplitOut).splits * heads * att_rows_padded(p) * 4, 256));
+  if (!backward && part > 0) l.part_lse = take(round_up((size_t)split_plan(p, kSplitOut).splits * heads * split_plan(p, kSplitOut).x_tiles * 512, 256));
   l.bytes = at;
   return l;
 }
@@ -148,7 +183,7 @@ static size_t forward_workspace(const FbevAttention& p) {
   if (!direct(p)) return split_layout(p, false).bytes;
   const AttPlan pl = attention_plan(p);
   if (pl.splits == 1) return 0;
-  return split_output_bytes(p, pl) + round_up((size_t)pl.splits * p.B * p.Hkv * att_rows_padded(p) * 4, 256);
+  return split_output_bytes(p, pl) + round_up((size_t)pl.splits * (p.B * p.Hkv * pl.row_blocks - pl.whole) * 256 * 4, 256);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -343,8 +378,9 @@ static int split_result(const FbevAttention& p, const SplitLayout& l, T* g, floa
   const int rc = p.D <= 64 ? split_launch<1, MODE>(p, l, pl, into, part, lse, st) : split_launch<2, MODE>(p, l, pl, into, part, lse, st);
   if (rc != FBEV_OK || whole) return rc;
   if (MODE == kSplitOut) {
-    launch_next(att_join_kernel<T>, (unsigned)((att_rows(p) * p.B * p.Hkv + 3) / 4), 128, 0, st, p, (const float*)part,
-                (const float*)reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + l.part_lse), pl.splits, g, lse);
+    const int units = p.B * p.Hkv * pl.x_tiles;
+    launch_next(att_join_kernel<T>, (unsigned)(units * 128), 128, 0, st, p,
+                JoinArgs{part, reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + l.part_lse), lse, pl.splits, 128, 0, units, pl.x_tiles, 128}, g);
   } else {
     const bool key_rows = MODE == kSplitDv || MODE == kSplitDk;
     const long long count = (long long)p.B * (key_rows ? (long long)p.Lk * p.Hkv : (long long)p.Lq * p.Hq) * p.D;
@@ -401,11 +437,12 @@ static int tensor_forward(const FbevAttention& p, T* out, float* lse, cudaStream
   a.c = score_factor(p);
   a.part = reinterpret_cast<float*>(p.workspace);
   a.part_lse = a.pl.splits > 1 ? reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + split_output_bytes(p, a.pl)) : nullptr;
-  const long long blocks = (long long)p.B * p.Hkv * a.pl.row_blocks * a.pl.splits;
-  att_fwd_kernel<T, NSUB><<<(unsigned)blocks, kAttThreads, AttFwdShape<NSUB>::kSmem, st>>>(a);
-  if (a.pl.splits > 1)
-    launch_next(att_join_kernel<T>, (unsigned)((att_rows(p) * p.B * p.Hkv + 3) / 4), 128, 0, st, p, (const float*)a.part,
-                (const float*)a.part_lse, a.pl.splits, out, lse);
+  const int units = p.B * p.Hkv * a.pl.row_blocks - a.pl.whole;  // split ones
+  const unsigned blocks = (unsigned)(a.pl.whole + units * a.pl.splits);
+  att_fwd_kernel<T, NSUB><<<blocks, kAttThreads, AttFwdShape<NSUB>::kSmem, st>>>(a);
+  if (units > 0)
+    launch_next(att_join_kernel<T>, (unsigned)(units * 256), 128, 0, st, p,
+                JoinArgs{a.part, a.part_lse, lse, a.pl.splits, 256, a.pl.whole, units, a.pl.row_blocks, a.pl.TL * a.pl.G}, out);
   return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
 }
 
@@ -425,12 +462,10 @@ static AttGradPlan gradient_plan(const FbevAttention& p, bool kv) {
   pl.TL = 128 / pl.G;
   pl.row_tiles = (p.Lq + pl.TL - 1) / pl.TL;
   pl.key_tiles = (p.Lk + 127) / 128;
-  const long long blocks = (long long)p.B * p.Hkv * (kv ? pl.key_tiles : pl.row_tiles);
-  const int other = kv ? pl.row_tiles : pl.key_tiles;
-  long long splits = blocks < kSms ? kSms / blocks : 1;
-  if (splits > other) splits = other;
-  pl.per_split = (int)((other + splits - 1) / splits);
-  pl.splits = (other + pl.per_split - 1) / pl.per_split;
+  const SplitChoice c = choose_splits(p.B * p.Hkv * (kv ? pl.key_tiles : pl.row_tiles), kv ? pl.row_tiles : pl.key_tiles,
+                                      (kv ? 2 : 1) * 128.0 * p.D * 4 / 40000.0, p.key_lengths != nullptr, false);
+  pl.splits = c.splits;
+  pl.per_split = c.per_split;
   return pl;
 }
 static size_t gradient_part_bytes(const FbevAttention& p, bool kv) {  // of one of the gradients
@@ -489,7 +524,7 @@ static int tensor_backward(const FbevAttention& p, const T* out, const float* ls
   const AttGradPlan pl = gradient_plan(p, false);
   float* nlse = reinterpret_cast<float*>(p.workspace);
   float* ndelta = reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + stat_bytes(p));
-  const unsigned blocks = (unsigned)((long long)p.B * p.Hkv * pl.row_tiles * 4);
+  const unsigned blocks = (unsigned)((long long)p.B * p.Hkv * pl.row_tiles);
   att_stat_kernel<T><<<blocks, 256, 0, st>>>(p, pl.TL, pl.row_tiles, out, go, lse, nlse, ndelta);
   int rc = cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
   if (rc == FBEV_OK && gq) rc = tensor_gradient<T, NSUB, false>(p, go, gq, (T*)nullptr, st);
