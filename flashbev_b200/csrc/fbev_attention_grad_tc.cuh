@@ -14,10 +14,11 @@
 // S and dP are formed twice that way, seven products instead of the least of five; in exchange nothing of dQ travels to
 // memory in float32 and the result is the same from run to run.
 //
-// A 128 x 128 tile of S is in the hands of eight warps, a thread has 64 columns of a row: tensor memory -> registers ->
-// P in 16 bits back over S (needed as an operand only for dV), then dP -> dS in 16 bits back over dP.  Each half of the
-// columns writes over its own half only.  While the warps form P of the next tile, the tensor cores run acc0 of this one
-// and dP of the next; while they form dS, acc1 and S of the next.
+// A 128 x 128 tile of S is in the hands of sixteen warps, a thread has 32 columns of a row: tensor memory -> registers ->
+// P in 16 bits back over S (needed as an operand only for dV), then dP -> dS in 16 bits back over dP.  Each quarter of the
+// columns writes over its own quarter only.  While the warps form P of the next tile, the tensor cores run acc0 of this one
+// and dP of the next; while they form dS, acc1 and S of the next.  All warps are in the same phase of a tile, so it is their
+// number that hides the latencies of a phase.
 //
 // Tensor memory, columns: S/P 0, dP/dS 128, acc0 256, acc1 384.
 #pragma once
@@ -44,6 +45,8 @@ struct AttGradArgs {
   float c;
 };
 
+constexpr int kGradThreads = 640;  // sixteen warps for P and dS, four for loads, matrix instructions and masks
+
 // two resident tiles and a ring of at least four: Y0 and Y1 of a tile are held while Y0 of the next is read
 template <int NSUB>
 struct AttGradShape {
@@ -53,7 +56,7 @@ struct AttGradShape {
 };
 
 template <typename T, int NSUB, bool KV>
-__global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_constant__ AttGradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_constant__ AttGradArgs a) {
   using Shape = AttGradShape<NSUB>;
   constexpr int kStages = Shape::kStages;
   constexpr uint32_t kStageBytes = Shape::kStageBytes;
@@ -100,14 +103,14 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     }
     mbar_init(x_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(p_done, 8);
+    mbar_init(p_done, 16);
     mbar_init(dp_full, 1);
-    mbar_init(ds_done, 8);
+    mbar_init(ds_done, 16);
     mbar_init(acc_full, 1);
     mbar_init(drained, 1);
     for (int i = 0; i < kMaskRing; ++i) {
       mbar_init(m_full(i), 1);
-      mbar_init(m_empty(i), 8);
+      mbar_init(m_empty(i), 16);
     }
     s_bail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,11 +118,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   if (KV && tile_rows < 128) {
     // rows that no load writes take part in the sums over rows: zeros instead of what the memory held
     for (int s = 0; s < kStages * NSUB; ++s)
-      for (int i = threadIdx.x; i < (128 - tile_rows) * 8; i += kAttThreads)
+      for (int i = threadIdx.x; i < (128 - tile_rows) * 8; i += kGradThreads)
         smem_zero16(s_ring + s * kTileBytes + tile_rows * 128 + i * 16);
     fence_async_smem();
   }
-  if (warp == 9) tmem_alloc<512>(&s_tmem);
+  if (warp == 17) tmem_alloc<512>(&s_tmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -130,9 +133,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   const auto needs_fix = [&](int t) { return fixes && (masked || (t0 + t + 1) * 128 > keys); };
   grid_dependency_wait();  // delta comes from the kernel before
 
-  if (warp >= 8) {
-    set_registers_down<80>();
-    if (warp == 8 && n > 0) {
+  if (warp >= 16) {
+    set_registers_down<64>();
+    if (warp == 16 && n > 0) {
       // ---- loads -------------------------------------------------------------------------------------------------
       const int qb = a.p.q_shared ? 0 : b;
       const auto load_rows = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int tile, int batch) {
@@ -169,7 +172,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         mbar_drain(x_full, 0);
         for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) mbar_drain(full(i % kStages), (i / kStages) & 1);
       }
-    } else if (warp == 9 && n > 0) {
+    } else if (warp == 17 && n > 0) {
       // ---- matrix instructions -----------------------------------------------------------------------------------
       const int ksteps = (a.p.D + 15) / 16;
       const uint32_t i_s = umma_instr<T>(128, false, a.p.scale < 0.0f), i_dp = umma_instr<T>(128, false, false),
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       const auto accumulate = [&](uint32_t d, uint32_t t, uint32_t y, bool first) {  // 16-bit tile in tensor memory times Y
         const uint64_t db = desc_mn_major(y);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) umma_ts(d, t + (k < 4 ? 8 * k : 32 + 8 * k), db + 128 * k, i_acc, !first || k > 0);
+        for (int k = 0; k < 8; ++k) umma_ts(d, t + 32 * (k / 2) + 8 * (k & 1), db + 128 * k, i_acc, !first || k > 0);
       };
       const auto scores = [&](int t) {
         wait_full(2 * t);
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         umma_commit(drained);
         mbar_drain(drained, 0);
       }
-    } else if (fixes && warp == 10 && n > 0) {
+    } else if (fixes && warp == 18 && n > 0) {
       // ---- key mask, keys that may not be attended -----------------------------------------------------------------
       const uint8_t* mask = masked ? a.p.key_mask + (long long)b * a.p.mask_stride : nullptr;
       const auto release = [&](int s) {
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         warp_wait(full(s1), ((2 * t + 1) / kStages) & 1, bail);
         release(s1);
       }
-    } else if (KV && warp == 10 && n > 0) {
+    } else if (KV && warp == 18 && n > 0) {
       // ---- statistics of the row tiles -----------------------------------------------------------------------------
       const float4* nlse = reinterpret_cast<const float4*>(a.nlse + ((long long)bg * pl.row_tiles + t0) * 128);
       const float4* ndelta = reinterpret_cast<const float4*>(a.ndelta + ((long long)bg * pl.row_tiles + t0) * 128);
@@ -289,10 +292,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     }
   } else {
     // ---- P and dS ----------------------------------------------------------------------------------------------------
-    set_registers_up<208>();
+    set_registers_up<104>();
     const int h = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = lanes + 64 * h, t_dp = lanes + 128 + 64 * h;
+    const uint32_t t_s = lanes + 32 * h, t_dp = lanes + 128 + 32 * h;
     const long long row = (long long)xt * tile_rows + r;             // dQ
     const bool row_live = !KV && r < tile_rows && row < rows;
     const int key = xt * 128 + r;                                    // dK, dV
@@ -300,25 +303,21 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     const float nd = KV ? 0.0f : a.ndelta[((long long)bg * pl.row_tiles + xt) * 128 + r];
     for (int t = 0; t < n; ++t) {
       const int mr = t % kMaskRing;
-      uint32_t word[2] = {kFull, kFull};
+      uint32_t word = kFull;
       if (!KV && masked) {
         warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
-        word[0] = s_mask[mr][2 * h];
-        word[1] = s_mask[mr][2 * h + 1];
+        word = s_mask[mr][h];
         __syncwarp();
         if (lane == 0) mbar_arrive(m_empty(mr));
       } else if (!KV && (t0 + t + 1) * 128 > keys) {
-        const int have = keys - (t0 + t) * 128 - 64 * h;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) word[x] = have >= 32 * x + 32 ? kFull : have <= 32 * x ? 0u : (1u << (have - 32 * x)) - 1u;
+        const int have = keys - (t0 + t) * 128 - 32 * h;
+        word = have >= 32 ? kFull : have <= 0 ? 0u : (1u << have) - 1u;
       }
-      const bool cut = (word[0] & word[1]) != kFull;
       warp_wait(s_full, t & 1, bail);
       if (KV) warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
       tc_fence_after();
-      float p[64];
+      float p[32];
       tmem_ld32(t_s, p);
-      tmem_ld32(t_s + 32, p + 32);
       tmem_wait_ld();
       if (!KV) {  // S may be overwritten
         tc_fence_before();
@@ -326,13 +325,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
         if (lane == 0) mbar_arrive(p_done);
       }
 #pragma unroll
-      for (int x = 0; x < 64; x += 16) {
+      for (int x = 0; x < 32; x += 16) {
         float2 e[8];
 #pragma unroll
         for (int y = 0; y < 8; y += 2) {
           const float* q = p + x + 2 * y;
           float4 l = make_float4(nl, nl, nl, nl);
-          if (KV) l = *reinterpret_cast<const float4*>(&s_stat[mr][0][64 * h + x + 2 * y]);
+          if (KV) l = *reinterpret_cast<const float4*>(&s_stat[mr][0][32 * h + x + 2 * y]);
           e[y] = fma2(make_float2(q[0], q[1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
           e[y + 1] = fma2(make_float2(q[2], q[3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
         }
@@ -343,11 +342,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
           p[x + 2 * y + 1] = e[y].y;
         }
       }
+      uint32_t packed[16];
       if (KV) {
-        uint32_t packed[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) packed[x] = pack2<T>(p[2 * x], p[2 * x + 1]);
-        tmem_st32(t_s, packed);
+        for (int x = 0; x < 16; ++x) packed[x] = pack2<T>(p[2 * x], p[2 * x + 1]);
+        __syncwarp();
+        tmem_st16(t_s, packed);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -355,32 +355,31 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
       }
       warp_wait(dp_full, t & 1, bail);
       tc_fence_after();
-      uint32_t packed[32];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        float dp[32];
-        tmem_ld32(t_dp + 32 * y, dp);
+        float dp[16];
+        tmem_ld16(t_dp + 16 * y, dp);
         tmem_wait_ld();
 #pragma unroll
-        for (int x = 0; x < 32; x += 4) {
+        for (int x = 0; x < 16; x += 4) {
           float4 d = make_float4(nd, nd, nd, nd);
-          if (KV) d = *reinterpret_cast<const float4*>(&s_stat[mr][1][64 * h + 32 * y + x]);
-          const float* q = p + 32 * y + x;
-          float2 s0 = add2(make_float2(dp[x], dp[x + 1]), make_float2(d.x, d.y));
-          float2 s1 = add2(make_float2(dp[x + 2], dp[x + 3]), make_float2(d.z, d.w));
-          s0 = make_float2(s0.x * q[0], s0.y * q[1]);
-          s1 = make_float2(s1.x * q[2], s1.y * q[3]);
-          if (cut) {  // a select, not a product: what stands there may be NaN
-            if (!((word[y] >> x) & 1)) s0.x = 0.0f;
-            if (!((word[y] >> (x + 1)) & 1)) s0.y = 0.0f;
-            if (!((word[y] >> (x + 2)) & 1)) s1.x = 0.0f;
-            if (!((word[y] >> (x + 3)) & 1)) s1.y = 0.0f;
+          if (KV) d = *reinterpret_cast<const float4*>(&s_stat[mr][1][32 * h + 16 * y + x]);
+          const float* q = p + 16 * y + x;
+          float2 s0 = mul2(add2(make_float2(dp[x], dp[x + 1]), make_float2(d.x, d.y)), make_float2(q[0], q[1]));
+          float2 s1 = mul2(add2(make_float2(dp[x + 2], dp[x + 3]), make_float2(d.z, d.w)), make_float2(q[2], q[3]));
+          if (word != kFull) {  // a select, not a product: what stands there may be NaN
+            const uint32_t w = word >> (16 * y + x);
+            if (!(w & 1)) s0.x = 0.0f;
+            if (!(w & 2)) s0.y = 0.0f;
+            if (!(w & 4)) s1.x = 0.0f;
+            if (!(w & 8)) s1.y = 0.0f;
           }
-          packed[16 * y + x / 2] = pack2<T>(s0.x, s0.y);
-          packed[16 * y + x / 2 + 1] = pack2<T>(s1.x, s1.y);
+          packed[8 * y + x / 2] = pack2<T>(s0.x, s0.y);
+          packed[8 * y + x / 2 + 1] = pack2<T>(s1.x, s1.y);
         }
       }
-      tmem_st32(t_dp, packed);
+      __syncwarp();
+      tmem_st16(t_dp, packed);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -391,7 +390,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     }
     if (n > 0) warp_wait(acc_full, 0, bail);
     tc_fence_after();
-    // ---- output: dQ column chunks in turn, or dK by the first group and dV by the second --------------------------------
+    // ---- output: a quarter of dQ's columns each, or dK by the even quarters and dV by the odd ones -------------------------
     const int d16 = (a.p.D + 15) / 16 * 16;
     const bool parted = pl.splits > 1;
     const bool live = KV ? key < a.p.Lk : row_live;
@@ -401,15 +400,16 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
     const long long at = KV ? (((long long)b * a.p.Lk + key) * a.p.Hkv + g) * a.p.D
                             : (((long long)b * a.p.Lq + l) * a.p.Hq + g * pl.G + (row - l * pl.G)) * a.p.D;
     const long long whole = KV ? (long long)a.p.B * a.p.Lk * a.p.Hkv * a.p.D : (long long)a.p.B * a.p.Lq * a.p.Hq * a.p.D;
-    T* dst = reinterpret_cast<T*>(KV && h ? a.g1 : a.g0) + at;
-    float* dpart = (KV && h ? a.part1 : a.part0) + split * whole + at;
-    const float f = KV && h ? 1.0f : a.p.scale;
+    const bool second = KV && (h & 1);
+    T* dst = reinterpret_cast<T*>(second ? a.g1 : a.g0) + at;
+    float* dpart = parted ? (second ? a.part1 : a.part0) + split * whole + at : nullptr;
+    const float f = second ? 1.0f : a.p.scale;
     __syncwarp();
 #pragma unroll 1
-    for (int x = KV ? 0 : 32 * h; x < d16; x += KV ? 32 : 64) {
+    for (int x = KV ? 32 * (h >> 1) : 32 * h; x < d16; x += KV ? 64 : 128) {
       float o[32];
       if (n > 0) {
-        tmem_ld32(lanes + (KV && h ? 384 : 256) + x, o);
+        tmem_ld32(lanes + (second ? 384 : 256) + x, o);
         tmem_wait_ld();
       }
       if (zero) {
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_grad_kernel(const __grid_c
   }
   grid_dependency_trigger();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_free<512>(s_tmem);
   }

@@ -604,20 +604,22 @@ struct JoinArgs {
   int whole, units;       // units before the first split one, split units
   int per_head;           // units of a (sample, key head)
   int tile_rows;          // rows of a row tile of 128
+  int warps;              // warps that share a row: 4 or 1
 };
 
-// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s: a block per row, its warps take the splits in
-// turn (in a fixed order) and add up in shared memory
+// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s.  Few rows: a block per row, whose warps take
+// the splits in turn (in a fixed order) and add up in shared memory; many: a warp per row.
 template <typename T>
 __global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ FbevAttention p, const __grid_constant__ JoinArgs a, T* __restrict__ out) {
   __shared__ float s_out[4][128], s_total[4];
   grid_dependency_wait();
-  const int u = blockIdx.x / a.slots, slot = blockIdx.x % a.slots;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int place = a.warps == 4 ? blockIdx.x : blockIdx.x * 4 + warp;
+  const int u = place / a.slots, slot = place % a.slots;
   const int unit = a.whole + u, bg = unit / a.per_head, G = p.Hq / p.Hkv;
   const long long rows = att_rows(p);
   const long long row = ((long long)(unit - bg * a.per_head) * (a.slots / 128) + slot / 128) * a.tile_rows + slot % 128;
-  if (slot % 128 >= a.tile_rows || row >= rows) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (slot % 128 >= a.tile_rows || row >= rows) return;  // the whole block where it shares a row
   const long long step = (long long)a.units * a.slots, at = (long long)u * a.slots + slot;
   float top = -INFINITY;
   for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_lse[s * step + at]);
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ F
   float total = 0.0f, o[4] = {};
   if (top != -INFINITY) {
 #pragma unroll 4
-    for (int s = warp; s < a.splits; s += 4) {
+    for (int s = a.warps == 4 ? warp : 0; s < a.splits; s += a.warps) {
       const float w = exp2_fast(a.part_lse[s * step + at] - top);
       const float* src = a.part + (s * step + at) * p.D;
       total += w;
@@ -635,19 +637,25 @@ __global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ F
         if (lane + 32 * i < p.D) o[i] = fmaf(w, src[lane + 32 * i], o[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s_out[warp][lane + 32 * i] = o[i];
-  if (lane == 0) s_total[warp] = total;
-  __syncthreads();
-  total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
-  const int c = threadIdx.x;
   const long long l = row / G;
   const int b = bg / p.Hkv, h = (bg % p.Hkv) * G + (int)(row - l * G);
-  if (c < p.D) {
+  T* dst = out + (((long long)b * p.Lq + l) * p.Hq + h) * p.D;
+  if (a.warps == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_out[warp][lane + 32 * i] = o[i];
+    if (lane == 0) s_total[warp] = total;
+    __syncthreads();
+    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+    const int c = threadIdx.x;
     const float v = (s_out[0][c] + s_out[1][c]) + (s_out[2][c] + s_out[3][c]);
-    out[(((long long)b * p.Lq + l) * p.Hq + h) * p.D + c] = from_float<T>(total == 0.0f ? 0.0f : v / total);
+    if (c < p.D) dst[c] = from_float<T>(total == 0.0f ? 0.0f : v / total);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < p.D) dst[lane + 32 * i] = from_float<T>(total == 0.0f ? 0.0f : o[i] / total);
   }
-  if (a.lse != nullptr && c == 0) a.lse[bg * att_rows_padded(p) + row] = total == 0.0f ? INFINITY : top + log2f(total);
+  if (a.lse != nullptr && lane == 0 && (warp == 0 || a.warps == 1))
+    a.lse[bg * att_rows_padded(p) + row] = total == 0.0f ? INFINITY : top + log2f(total);
 }
 
 }  // namespace fbev

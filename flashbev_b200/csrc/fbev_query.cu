@@ -111,7 +111,8 @@ static AttPlan attention_plan(const FbevAttention& p) {
   pl.pair = pl.row_tiles == 1;
   pl.row_blocks = (pl.row_tiles + 1) / 2;
   const int units = p.B * p.Hkv * pl.row_blocks, key_tiles = (p.Lk + 127) / 128;
-  const SplitChoice c = choose_splits(units, key_tiles, 0.5 * pl.G * pl.TL * 2 * p.D * 4 / 40000.0, p.key_lengths != nullptr, true);
+  // few rows: the memory's rate bounds a step, and splitting only pays to give every SM work
+  const SplitChoice c = choose_splits(units, key_tiles, 256.0 * p.D * 4 / 40000.0, p.key_lengths != nullptr && !pl.pair, !pl.pair);
   pl.whole = c.whole;
   pl.splits = c.splits;
   pl.per_split = c.per_split;
@@ -277,6 +278,14 @@ static float score_factor(const FbevAttention& p) {
   return c < 1e-30f ? 1e-30f : c;
 }
 
+// a block per row where that still leaves the GPU room, else a warp
+template <typename T>
+static void launch_join(const FbevAttention& p, JoinArgs a, T* out, cudaStream_t st) {
+  const int places = a.units * a.slots;
+  a.warps = a.splits > 4 && places <= kSms * 16 ? 4 : 1;
+  launch_next(att_join_kernel<T>, (unsigned)(a.warps == 4 ? places : places / 4), 128, 0, st, p, a, out);
+}
+
 // ---- three-part operands: launches -------------------------------------------------------------------------------------
 
 static int encode_parts(CUtensorMap* map, const void* ptr, long long rows, long long heads, int width) {
@@ -379,8 +388,8 @@ static int split_result(const FbevAttention& p, const SplitLayout& l, T* g, floa
   if (rc != FBEV_OK || whole) return rc;
   if (MODE == kSplitOut) {
     const int units = p.B * p.Hkv * pl.x_tiles;
-    launch_next(att_join_kernel<T>, (unsigned)(units * 128), 128, 0, st, p,
-                JoinArgs{part, reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + l.part_lse), lse, pl.splits, 128, 0, units, pl.x_tiles, 128}, g);
+    launch_join<T>(p, JoinArgs{part, reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + l.part_lse), lse, pl.splits, 128, 0, units,
+                               pl.x_tiles, 128, 0}, g, st);
   } else {
     const bool key_rows = MODE == kSplitDv || MODE == kSplitDk;
     const long long count = (long long)p.B * (key_rows ? (long long)p.Lk * p.Hkv : (long long)p.Lq * p.Hq) * p.D;
@@ -441,8 +450,7 @@ static int tensor_forward(const FbevAttention& p, T* out, float* lse, cudaStream
   const unsigned blocks = (unsigned)(a.pl.whole + units * a.pl.splits);
   att_fwd_kernel<T, NSUB><<<blocks, kAttThreads, AttFwdShape<NSUB>::kSmem, st>>>(a);
   if (units > 0)
-    launch_next(att_join_kernel<T>, (unsigned)(units * 256), 128, 0, st, p,
-                JoinArgs{a.part, a.part_lse, lse, a.pl.splits, 256, a.pl.whole, units, a.pl.row_blocks, a.pl.TL * a.pl.G}, out);
+    launch_join<T>(p, JoinArgs{a.part, a.part_lse, lse, a.pl.splits, 256, a.pl.whole, units, a.pl.row_blocks, a.pl.TL * a.pl.G, 0}, out, st);
   return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
 }
 
@@ -508,7 +516,7 @@ static int tensor_gradient(const FbevAttention& p, const T* go, T* g0, T* g1, cu
   a.g1 = g1;
   a.c = score_factor(p);
   const long long blocks = (long long)p.B * p.Hkv * (KV ? a.pl.key_tiles : a.pl.row_tiles) * a.pl.splits;
-  launch_next(att_grad_kernel<T, NSUB, KV>, (unsigned)blocks, kAttThreads, AttGradShape<NSUB>::kSmem, st, a);
+  launch_next(att_grad_kernel<T, NSUB, KV>, (unsigned)blocks, kGradThreads, AttGradShape<NSUB>::kSmem, st, a);
   if (a.pl.splits > 1) {
     const long long count = (long long)p.B * (KV ? (long long)p.Lk * p.Hkv : (long long)p.Lq * p.Hq) * p.D;
     const long long want = (count + 255) / 256;
