@@ -313,8 +313,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         const int have = keys - (t0 + t) * 128 - 32 * h;
         word = have >= 32 ? kFull : have <= 0 ? 0u : (1u << have) - 1u;
       }
+      // the columns' statistics: read before the wait, while the tensor cores leave shared memory some room
+      float4 col[KV ? 8 : 1];
+      if (KV) {
+        warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) col[x] = *reinterpret_cast<const float4*>(&s_stat[mr][0][32 * h + 4 * x]);
+      }
       warp_wait(s_full, t & 1, bail);
-      if (KV) warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
       tc_fence_after();
       float p[32];
       tmem_ld32(t_s, p);
@@ -331,7 +337,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         for (int y = 0; y < 8; y += 2) {
           const float* q = p + x + 2 * y;
           float4 l = make_float4(nl, nl, nl, nl);
-          if (KV) l = *reinterpret_cast<const float4*>(&s_stat[mr][0][32 * h + x + 2 * y]);
+          if (KV) l = col[(x + 2 * y) / 4];
           e[y] = fma2(make_float2(q[0], q[1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
           e[y + 1] = fma2(make_float2(q[2], q[3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
         }
@@ -353,6 +359,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(p_done);
       }
+      if (KV) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) col[x] = *reinterpret_cast<const float4*>(&s_stat[mr][1][32 * h + 4 * x]);
+      }
       warp_wait(dp_full, t & 1, bail);
       tc_fence_after();
 #pragma unroll
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
 #pragma unroll
         for (int x = 0; x < 16; x += 4) {
           float4 d = make_float4(nd, nd, nd, nd);
-          if (KV) d = *reinterpret_cast<const float4*>(&s_stat[mr][1][32 * h + 16 * y + x]);
+          if (KV) d = col[4 * y + x / 4];
           const float* q = p + 16 * y + x;
           float2 s0 = mul2(add2(make_float2(dp[x], dp[x + 1]), make_float2(d.x, d.y)), make_float2(q[0], q[1]));
           float2 s1 = mul2(add2(make_float2(dp[x + 2], dp[x + 3]), make_float2(d.z, d.w)), make_float2(q[2], q[3]));

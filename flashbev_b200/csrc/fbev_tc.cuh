@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)
 // A value that is the same in all lanes, told so to the compiler: what the roles' loops are bounded and addressed by stays in
 // uniform registers.  Loops that look as if lanes could part would have every matrix instruction go through a search for
 // the lanes that issue it (measured: 1700 clocks for the dozen instructions of a step, longer than the step itself).
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(kFull, v, 0); }
+__device__ __forceinline__ int uniform(int v) { return (int)__reduce_max_sync(kFull, (unsigned)v); }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -46,28 +46,34 @@ struct Bail {
   uint32_t* status;
 };
 
-// Waits until the phase of the given parity has completed.  Gives up after about two seconds, or soon after another thread
-// of the block did.  Nothing is returned: a block that gave up runs its loops to their end with whatever it has, all its
-// accesses being in bounds whatever the data, and the status word tells that the result is not valid.
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
-  if (mbar_try(bar, parity)) return;
+// A run of tries, in one piece of text: to the compiler the code around it has no branch that lanes could part at.
+__device__ __forceinline__ bool mbar_try_run(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p, q;\n.reg .u32 i;\nmov.u32 i, 0;\n"
+      "AGAIN:\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n@p bra DONE;\n"
+      "add.u32 i, i, 1;\nsetp.lt.u32 q, i, 1024;\n@q bra AGAIN;\nDONE:\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// Waits, as a whole warp, until the phase of the given parity has completed.  Gives up after about two seconds, or soon
+// after another warp of the block did.  Nothing is returned: a block that gave up runs its loops to their end with whatever
+// it has, all its accesses being in bounds whatever the data, and the status word tells that the result is not valid.
+__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
+  if (__all_sync(kFull, mbar_try_run(bar, parity))) return;
   const long long t0 = clock64();
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-      if (mbar_try(bar, parity)) return;
-    if (*bail.flag != 0) return;
-    if (clock64() - t0 > 4000000000ll) {
+  while (!__all_sync(kFull, mbar_try(bar, parity))) {
+    if (__any_sync(kFull, *bail.flag != 0)) return;
+    if (__any_sync(kFull, clock64() - t0 > 4000000000ll)) {
       *bail.flag = 1;
-      if (bail.status != nullptr) atomicOr(bail.status, (uint32_t)FBEV_DEV_TIMEOUT);
+      if (bail.status != nullptr && (threadIdx.x & 31) == 0) atomicOr(bail.status, (uint32_t)FBEV_DEV_TIMEOUT);
+      __syncwarp();
       return;
     }
   }
-}
-// the same for a whole warp, which is together afterwards
-__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, const Bail& bail) {
-  mbar_wait(bar, parity, bail);
-  __syncwarp();
 }
 // for a while only, whatever became of the others: before a block that gave up ends
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
