@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .flash_bevpool import _DTYPES, _on_device, status_word
+from .flash_bevpool import _DTYPES, status_word
 
 _POS_DTYPES = {torch.float32: _lib.POS_F32, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
 
@@ -38,8 +38,36 @@ def _check_tensor(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = Non
                          f"got {t.dtype}, {t.device}")
 
 
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index; the handle without a Stream object around it
+
+
+class _on:
+    """Makes a device index current for the launch; costs nothing to speak of when it is already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, index: int):
+        self.guard = None if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+# What a call needs that follows from sizes, strides and types alone (checks passed, the filled C struct without its
+# addresses, workspace sizes) is worked out once per such signature.  At most this many are kept of each operator.
+_MOST_PLANS = 512
+
+
+def _remember(plans: dict, key, plan):
+    if len(plans) >= _MOST_PLANS:
+        plans.clear()
+    plans[key] = plan
+    return plan
 
 
 def _operand(t: torch.Tensor, shared_batch: bool = False) -> torch.Tensor:
@@ -55,7 +83,20 @@ def _operand(t: torch.Tensor, shared_batch: bool = False) -> torch.Tensor:
     return t if good else t.clone(memory_format=torch.contiguous_format)
 
 
-def _attention_problem(q, k, v, lengths, mask, scale):
+class _AttentionPlan:
+    __slots__ = ("template", "workspace", "lse_count", "index")
+
+
+_attention_plans: dict = {}
+
+
+def _attention_plan(q, k, v, lengths, mask, scale) -> _AttentionPlan:
+    """Of operands that _operand has been through."""
+    key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), q.dtype, q.device, lengths is None,
+           None if mask is None else mask.stride(0), scale)
+    plan = _attention_plans.get(key)
+    if plan is not None:
+        return plan
     p = _lib.FbevAttention()
     p.struct_size = ctypes.sizeof(_lib.FbevAttention)
     p.dtype = _DTYPES[q.dtype]
@@ -66,35 +107,46 @@ def _attention_problem(q, k, v, lengths, mask, scale):
     p.q_stride[:] = q.stride()[:3]
     p.k_stride[:] = k.stride()[:3]
     p.v_stride[:] = v.stride()[:3]
+    p.mask_stride = 0 if mask is None or p.B == 1 else mask.stride(0)
+    p.status = status_word(q.device).data_ptr()
+    # sizes depend on the addresses' alignment, which _operand has seen to, and on whether there are lengths
+    p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if lengths is not None:
+        p.key_lengths = lengths.data_ptr()
+    lib = _lib.load()
+    plan = _AttentionPlan()
+    plan.workspace = tuple(lib.fbev_cross_attention_workspace_bytes(ctypes.byref(p), i) for i in (0, 1))
+    plan.lse_count = lib.fbev_cross_attention_lse_count(ctypes.byref(p))
+    plan.index = q.device.index
+    p.q = p.k = p.v = p.key_lengths = None
+    plan.template = bytes(p)
+    return _remember(_attention_plans, key, plan)
+
+
+def _attention_problem(plan, q, k, v, lengths, mask, backward):
+    """The filled struct and the workspace, which has to live until the launch is queued."""
+    p = _lib.FbevAttention.from_buffer_copy(plan.template)
     p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if lengths is not None:
         p.key_lengths = lengths.data_ptr()
     if mask is not None:
-        p.key_mask, p.mask_stride = mask.data_ptr(), mask.stride(0) if p.B > 1 else 0
-    p.status = status_word(q.device).data_ptr()
-    return p
-
-
-def _attention_workspace(lib, p, backward: bool, device: torch.device):
-    nbytes = lib.fbev_cross_attention_workspace_bytes(ctypes.byref(p), 1 if backward else 0)
+        p.key_mask = mask.data_ptr()
+    nbytes = plan.workspace[backward]
     if not nbytes:
-        return None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return p, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
-    return ws
+    return p, ws
 
 
 def _attention_forward(q, k, v, lengths, mask, scale, with_lse):
-    lib = _lib.load()
-    dev = q.device
-    with _on_device(dev):
-        p = _attention_problem(q, k, v, lengths, mask, scale)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        lse = None
-        if with_lse:
-            lse = torch.empty(lib.fbev_cross_attention_lse_count(ctypes.byref(p)), dtype=torch.float32, device=dev)
-        ws = _attention_workspace(lib, p, False, dev)  # noqa: F841 - alive until the launch is queued
-        rc = lib.fbev_cross_attention(ctypes.byref(p), out.data_ptr(), lse.data_ptr() if with_lse else None, _stream(dev))
+    plan = _attention_plan(q, k, v, lengths, mask, scale)
+    with _on(plan.index):
+        p, ws = _attention_problem(plan, q, k, v, lengths, mask, 0)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(plan.lse_count, dtype=torch.float32, device=q.device) if with_lse else None
+        rc = _lib.load().fbev_cross_attention(ctypes.byref(p), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                              _stream(plan.index))
     if rc:
         _lib.check(rc, "fbev_cross_attention")
     return out, lse
@@ -112,24 +164,23 @@ class _CrossAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         q, k, v, lengths, mask, out, lse = ctx.saved_tensors
-        lib = _lib.load()
         dev = q.device
         need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         gq = gk = gv = None
-        with _on_device(dev):
+        plan = _attention_plan(q, k, v, lengths, mask, ctx.scale)
+        with _on(plan.index):
             go = grad_out.contiguous()
             if go.data_ptr() % 16:
                 go = go.clone()
-            p = _attention_problem(q, k, v, lengths, mask, ctx.scale)
+            p, ws = _attention_problem(plan, q, k, v, lengths, mask, 1)
             if need_q:
                 gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
             if need_kv:
                 gk = torch.empty(k.shape, dtype=k.dtype, device=dev)
                 gv = torch.empty(v.shape, dtype=v.dtype, device=dev)
-            ws = _attention_workspace(lib, p, True, dev)  # noqa: F841
-            rc = lib.fbev_cross_attention_grad(ctypes.byref(p), out.data_ptr(), lse.data_ptr(), go.data_ptr(),
-                                               gq.data_ptr() if need_q else None, gk.data_ptr() if need_kv else None,
-                                               gv.data_ptr() if need_kv else None, _stream(dev))
+            rc = _lib.load().fbev_cross_attention_grad(
+                ctypes.byref(p), out.data_ptr(), lse.data_ptr(), go.data_ptr(), gq.data_ptr() if need_q else None,
+                gk.data_ptr() if need_kv else None, gv.data_ptr() if need_kv else None, _stream(plan.index))
         if rc:
             _lib.check(rc, "fbev_cross_attention_grad")
         return (gq, gk if ctx.needs_input_grad[1] else None, gv if ctx.needs_input_grad[2] else None, None, None, None)
@@ -155,16 +206,39 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     type before they meet the values, as are the score gradients before they meet queries and keys.  Gradients are the
     same from run to run.  With few queries the keys are split over the GPU and the parts joined.
     """
+    # the checks pass once per combination of shapes, types and devices
+    key = (q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, q.device, k.device, v.device)
+    if key not in _attention_checked:
+        _check_attention(q, k, v)
+        _remember(_attention_checked, key, True)
+    if key_lengths is not None or key_mask is not None:
+        key_lengths, key_mask = _attention_masks(q, k, key_lengths, key_mask)
+    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossAttention.apply(q, k, v, key_lengths, key_mask, scale)
+    return _attention_forward(q, k, v, key_lengths, key_mask, scale, False)[0]
+
+
+_attention_checked: dict = {}
+
+
+def _check_attention(q, k, v) -> None:
     _check_tensor("q", q)
     _check_tensor("k", k, q)
     _check_tensor("v", v, q)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q must be [B,Lq,Hq,D] and k, v [B,Lk,Hkv,D]; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    B, Lk, D = q.shape[0], k.shape[1], q.shape[3]
-    if not 1 <= D <= 128:
-        raise ValueError(f"the head width must be 1 to 128, got {D}")
+    if not 1 <= q.shape[3] <= 128:
+        raise ValueError(f"the head width must be 1 to 128, got {q.shape[3]}")
     if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2] != 0:
         raise ValueError(f"the number of query heads ({q.shape[2]}) must be a multiple of the key heads ({k.shape[2]})")
+
+
+def _attention_masks(q, k, key_lengths, key_mask):
+    B, Lk = k.shape[:2]
     if key_lengths is not None:
         if key_lengths.shape != (B,) or key_lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"key_lengths must be int32 or int64 of shape [{B}]")
@@ -179,13 +253,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
             key_mask = key_mask.unsqueeze(0).expand(B, Lk)
         if Lk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-    q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CrossAttention.apply(q, k, v, key_lengths, key_mask, scale)
-    return _attention_forward(q, k, v, key_lengths, key_mask, scale, False)[0]
+    return key_lengths, key_mask
 
 
 @functools.lru_cache(maxsize=64)
@@ -200,23 +268,30 @@ def _rotary_table(sections, base):
     return turns, axis
 
 
+_rotary_plans: dict = {}
+
+
 def _rotary(x, positions, sections, base, interleaved, inverse):
-    lib = _lib.load()
-    dev = x.device
-    p = _lib.FbevRotary()
-    p.struct_size = ctypes.sizeof(_lib.FbevRotary)
-    p.dtype = _DTYPES[x.dtype]
-    p.B, p.L, p.H, p.D = x.shape
-    p.pairs, p.axes = sum(sections), len(sections)
-    p.interleaved, p.inverse = int(interleaved), int(inverse)
-    p.pos_dtype = _POS_DTYPES[positions.dtype]
-    p.x_stride[:] = x.stride()[:3]
-    p.pos_stride = 0 if positions.dim() == 2 else positions.stride(0)
+    key = (x.shape, x.stride(), x.dtype, positions.dtype, positions.dim(), sections, base, interleaved, inverse)
+    template = _rotary_plans.get(key)
+    if template is None:
+        p = _lib.FbevRotary()
+        p.struct_size = ctypes.sizeof(_lib.FbevRotary)
+        p.dtype = _DTYPES[x.dtype]
+        p.B, p.L, p.H, p.D = x.shape
+        p.pairs, p.axes = sum(sections), len(sections)
+        p.interleaved, p.inverse = int(interleaved), int(inverse)
+        p.pos_dtype = _POS_DTYPES[positions.dtype]
+        p.x_stride[:] = x.stride()[:3]
+        p.pos_stride = 0 if positions.dim() == 2 else positions.stride(0)
+        p.pair_turns, p.pair_axis = _rotary_table(sections, base)
+        template = _remember(_rotary_plans, key, bytes(p))
+    p = _lib.FbevRotary.from_buffer_copy(template)
     p.x, p.positions = x.data_ptr(), positions.data_ptr()
-    p.pair_turns, p.pair_axis = _rotary_table(sections, base)
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    with _on_device(dev):
-        rc = lib.fbev_rotary_axes(ctypes.byref(p), out.data_ptr(), _stream(dev))
+    index = x.device.index
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(index):
+        rc = _lib.load().fbev_rotary_axes(ctypes.byref(p), out.data_ptr(), _stream(index))
     if rc:
         _lib.check(rc, "fbev_rotary_axes")
     return out
@@ -262,27 +337,14 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, sections: Sequence[int
 
     Angles are reduced in float64, so far positions keep their full accuracy.
     """
-    _check_tensor("x", x)
-    if x.dim() != 4 or not 1 <= x.shape[3] <= 256:
-        raise ValueError(f"x must be [B,L,H,D] with D from 1 to 256, got {tuple(x.shape)}")
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= 8 or min(sections) < 0 or 2 * sum(sections) > x.shape[3]:
-        raise ValueError(f"sections must be 1 to 8 non-negative numbers with 2 * sum <= {x.shape[3]}, got {sections}")
-    B, L = x.shape[:2]
-    if positions.shape not in ((L, len(sections)), (B, L, len(sections))):
-        raise ValueError(f"positions must be [{L},{len(sections)}] or [{B},{L},{len(sections)}], got {tuple(positions.shape)}")
-    if positions.dtype not in _POS_DTYPES:
-        raise ValueError(f"positions must be float32, int32 or int64, got {positions.dtype}")
+    sections = tuple(sections)
+    key = (x.shape, x.dtype, x.device, positions.shape, positions.dtype, positions.device, sections, base, interleaved)
+    if key not in _rotary_checked:
+        _check_rotary(x, positions, sections, base, interleaved)
+        _remember(_rotary_checked, key, True)
     if positions.requires_grad:
         raise ValueError("positions carry no gradient; detach them")
-    if positions.device != x.device:
-        raise ValueError("positions are on another device than x")
-    base = float(base)
-    if not (math.isfinite(base) and base > 0):
-        raise ValueError("base must be positive and finite")
-    interleaved = bool(interleaved)
-    if interleaved and x.shape[3] % 2:
-        raise ValueError("interleaved pairs need an even D")
+    base, interleaved = float(base), bool(interleaved)
     positions = positions.contiguous()
     x = _rotary_operand(x, interleaved)
     if torch.is_grad_enabled() and x.requires_grad:
@@ -290,21 +352,43 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, sections: Sequence[int
     return _rotary(x, positions, sections, base, interleaved, False)
 
 
+_rotary_checked: dict = {}
+
+
+def _check_rotary(x, positions, sections, base, interleaved) -> None:
+    _check_tensor("x", x)
+    if x.dim() != 4 or not 1 <= x.shape[3] <= 256:
+        raise ValueError(f"x must be [B,L,H,D] with D from 1 to 256, got {tuple(x.shape)}")
+    if not all(isinstance(s, int) for s in sections) or not 1 <= len(sections) <= 8 or min(sections) < 0 \
+            or 2 * sum(sections) > x.shape[3]:
+        raise ValueError(f"sections must be 1 to 8 non-negative whole numbers with 2 * sum <= {x.shape[3]}, got {sections}")
+    B, L = x.shape[:2]
+    if positions.shape not in ((L, len(sections)), (B, L, len(sections))):
+        raise ValueError(f"positions must be [{L},{len(sections)}] or [{B},{L},{len(sections)}], got {tuple(positions.shape)}")
+    if positions.dtype not in _POS_DTYPES:
+        raise ValueError(f"positions must be float32, int32 or int64, got {positions.dtype}")
+    if positions.device != x.device:
+        raise ValueError("positions are on another device than x")
+    if not (math.isfinite(base) and base > 0):
+        raise ValueError("base must be positive and finite")
+    if interleaved and x.shape[3] % 2:
+        raise ValueError("interleaved pairs need an even D")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
 def _norm_forward(x, residual, weight, eps, with_rstd):
-    lib = _lib.load()
     C = x.shape[-1]
     rows = x.numel() // C
-    dev = x.device
+    index = x.device.index
     y = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if with_rstd else None
-    with _on_device(dev):
-        rc = lib.fbev_add_rms_norm(_DTYPES[x.dtype], rows, C, eps, x.data_ptr(), _ptr(residual), _ptr(weight), y.data_ptr(),
-                                   _ptr(h), _ptr(rstd), _stream(dev))
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if with_rstd else None
+    with _on(index):
+        rc = _lib.load().fbev_add_rms_norm(_DTYPES[x.dtype], rows, C, eps, x.data_ptr(), _ptr(residual), _ptr(weight),
+                                           y.data_ptr(), _ptr(h), _ptr(rstd), _stream(index))
     if rc:
         _lib.check(rc, "fbev_add_rms_norm")
     return y, h, rstd
@@ -330,7 +414,7 @@ class _AddRmsNorm(torch.autograd.Function):
         dev = h.device
         need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         need_w = ctx.needs_input_grad[2]
-        with _on_device(dev):
+        with _on(dev.index):
             grad_y = grad_y.contiguous()
             grad_h = None if grad_h is None else grad_h.contiguous()
             gx = torch.empty_like(h) if need_x else None
@@ -339,7 +423,7 @@ class _AddRmsNorm(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             rc = lib.fbev_add_rms_norm_grad(_DTYPES[h.dtype], rows, C, h.data_ptr(), rstd.data_ptr(), _ptr(weight),
                                             grad_y.data_ptr(), _ptr(grad_h), _ptr(gx), _ptr(gw), _ptr(ws), nbytes,
-                                            _stream(dev))
+                                            _stream(dev.index))
         if rc:
             _lib.check(rc, "fbev_add_rms_norm_grad")
         return (gx if ctx.needs_input_grad[0] else None, gx if ctx.needs_input_grad[1] else None, gw, None)
@@ -359,24 +443,18 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
         (y, h), or (q, scales, h) with ``quantize``: q like y in float8_e4m3fn, scales [...] float32, y ~ q * scales.
         Without a residual h is x itself.
     """
-    _check_tensor("x", x)
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 20:
-        raise ValueError(f"x must be [..., C] with C from 1 to 2^20, got {tuple(x.shape)}")
-    if residual is not None:
-        _check_tensor("residual", residual, x)
-        if residual.shape != x.shape:
-            raise ValueError(f"residual must have the shape of x {tuple(x.shape)}, got {tuple(residual.shape)}")
-        residual = residual.contiguous()
-    if weight is not None:
-        _check_tensor("weight", weight, x)
-        if weight.shape != x.shape[-1:]:
-            raise ValueError(f"weight must have shape [{x.shape[-1]}], got {tuple(weight.shape)}")
-        weight = weight.contiguous()
-    x = x.contiguous()
-    eps = float(eps)
-    if not (math.isfinite(eps) and eps >= 0):
+    key = (x.shape, x.dtype, x.device, None if residual is None else (residual.shape, residual.dtype, residual.device),
+           None if weight is None else (weight.shape, weight.dtype, weight.device))
+    if key not in _norm_checked:
+        _check_norm(x, residual, weight)
+        _remember(_norm_checked, key, True)
+    if not 0.0 <= eps < math.inf:
         raise ValueError("eps must be finite and not negative")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight))
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    grad = torch.is_grad_enabled() and (
+        x.requires_grad or (residual is not None and residual.requires_grad) or (weight is not None and weight.requires_grad))
     if quantize:
         if grad:
             raise ValueError("the 8-bit output carries no gradient; call under torch.no_grad()")
@@ -386,9 +464,9 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
         q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
         scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
         h = torch.empty_like(x) if residual is not None else None
-        with _on_device(dev):
+        with _on(dev.index):
             rc = lib.fbev_add_rms_norm_e4m3(_DTYPES[x.dtype], x.numel() // C, C, eps, x.data_ptr(), _ptr(residual), _ptr(weight),
-                                            q.data_ptr(), scales.data_ptr(), _ptr(h), _stream(dev))
+                                            q.data_ptr(), scales.data_ptr(), _ptr(h), _stream(dev.index))
         if rc:
             _lib.check(rc, "fbev_add_rms_norm_e4m3")
         return q, scales, x if h is None else h
@@ -398,3 +476,20 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
     if residual is None:
         return _AddRmsNorm.apply(x, None, weight, eps), x
     return _AddRmsNorm.apply(x, residual, weight, eps)
+
+
+_norm_checked: dict = {}
+
+
+def _check_norm(x, residual, weight) -> None:
+    _check_tensor("x", x)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 20:
+        raise ValueError(f"x must be [..., C] with C from 1 to 2^20, got {tuple(x.shape)}")
+    if residual is not None:
+        _check_tensor("residual", residual, x)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must have the shape of x {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if weight is not None:
+        _check_tensor("weight", weight, x)
+        if weight.shape != x.shape[-1:]:
+            raise ValueError(f"weight must have shape [{x.shape[-1]}], got {tuple(weight.shape)}")
