@@ -194,20 +194,28 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(const __grid_co
     const int c = (n * LANES + lane) * VE;
     if (w && c < a.C) pw[n] = *reinterpret_cast<const Pack<T, VE>*>(w + c);
   }
-  for (long long first = (long long)blockIdx.x * kGroups; first < a.rows; first += (long long)gridDim.x * kGroups) {
-    const long long row = first + group;
-    const bool live = row < a.rows;
-    const long long base = row * a.C;
-    Pack<T, VE> ph[NV], py[NV], pd[NV];
-    const float s = live ? a.rstd_in[row] : 0.0f;
+  // the next row travels while this one is summed up
+  Pack<T, VE> ph[NV], py[NV], pd[NV];
+  float s = 0.0f;
+  const auto fetch = [&](long long row) {
+    if (row >= a.rows) return;
+    s = a.rstd_in[row];
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int c = (n * LANES + lane) * VE;
-      if (!live || c >= a.C) continue;
-      ph[n] = *reinterpret_cast<const Pack<T, VE>*>(hp + base + c);
-      if (dy) py[n] = *reinterpret_cast<const Pack<T, VE>*>(dy + base + c);
-      if (dh) pd[n] = *reinterpret_cast<const Pack<T, VE>*>(dh + base + c);
+      if (c >= a.C) continue;
+      ph[n] = *reinterpret_cast<const Pack<T, VE>*>(hp + row * a.C + c);
+      if (dy) py[n] = *reinterpret_cast<const Pack<T, VE>*>(dy + row * a.C + c);
+      if (dh) pd[n] = *reinterpret_cast<const Pack<T, VE>*>(dh + row * a.C + c);
     }
+  };
+  const long long stride = (long long)gridDim.x * kGroups;
+  fetch((long long)blockIdx.x * kGroups + group);
+  for (long long first = (long long)blockIdx.x * kGroups; first < a.rows; first += stride) {
+    const long long row = first + group;
+    const bool live = row < a.rows;
+    const long long base = row * a.C;
+    const float rs = s;
     float dot = 0.0f;
     float nv[NV][VE], g[NV][VE];  // n and w dy
 #pragma unroll
@@ -216,13 +224,17 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(const __grid_co
       const bool in = live && c < a.C;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        nv[n][e] = in ? to_float(ph[n].v[e]) * s : 0.0f;
+        nv[n][e] = in ? to_float(ph[n].v[e]) * rs : 0.0f;
         const float d = in && dy ? to_float(py[n].v[e]) : 0.0f;
         dw[n][e] = fmaf(d, nv[n][e], dw[n][e]);
         g[n][e] = in && w ? d * to_float(pw[n].v[e]) : d;
         dot = fmaf(g[n][e], nv[n][e], dot);
       }
     }
+    Pack<T, VE> up[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) up[n] = pd[n];
+    fetch(row + stride);
     if (!a.dx) continue;  // uniform
     dot = group_reduce<LANES, false>(dot, red) / (float)a.C;
 #pragma unroll
@@ -232,7 +244,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(const __grid_co
       Pack<T, VE> po;
 #pragma unroll
       for (int e = 0; e < VE; ++e)
-        po.v[e] = from_float<T>(fmaf(s, fmaf(-nv[n][e], dot, g[n][e]), dh ? to_float(pd[n].v[e]) : 0.0f));
+        po.v[e] = from_float<T>(fmaf(rs, fmaf(-nv[n][e], dot, g[n][e]), dh ? to_float(up[n].v[e]) : 0.0f));
       *reinterpret_cast<Pack<T, VE>*>(reinterpret_cast<T*>(a.dx) + base + c) = po;
     }
   }
@@ -294,6 +306,7 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* __restrict__
   const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, g = threadIdx.x >> 5;
   float v = 0.0f;
   if (c < C)
+#pragma unroll 8
     for (int i = g; i < blocks; i += 32) v += part[(long long)i * C + c];
   s[g][lane] = v;
   __syncthreads();
