@@ -177,8 +177,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_long_kernel(const __grid_co
   }
 }
 
+// A row's values are unpacked twice rather than kept unpacked: four blocks of one chunk a lane fit an SM then (the grid is
+// that many), and what hides the memory's latency here is their number.
 template <typename T, int VE, int NV, int LANES>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : NV == 2 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[kNormThreads / 32];
   extern __shared__ float s_dw[];  // [C], only with dw_part
   constexpr int kGroups = kNormThreads / LANES;
@@ -194,47 +196,32 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(const __grid_co
     const int c = (n * LANES + lane) * VE;
     if (w && c < a.C) pw[n] = *reinterpret_cast<const Pack<T, VE>*>(w + c);
   }
-  // the next row travels while this one is summed up
-  Pack<T, VE> ph[NV], py[NV], pd[NV];
-  float s = 0.0f;
-  const auto fetch = [&](long long row) {
-    if (row >= a.rows) return;
-    s = a.rstd_in[row];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int c = (n * LANES + lane) * VE;
-      if (c >= a.C) continue;
-      ph[n] = *reinterpret_cast<const Pack<T, VE>*>(hp + row * a.C + c);
-      if (dy) py[n] = *reinterpret_cast<const Pack<T, VE>*>(dy + row * a.C + c);
-      if (dh) pd[n] = *reinterpret_cast<const Pack<T, VE>*>(dh + row * a.C + c);
-    }
-  };
-  const long long stride = (long long)gridDim.x * kGroups;
-  fetch((long long)blockIdx.x * kGroups + group);
-  for (long long first = (long long)blockIdx.x * kGroups; first < a.rows; first += stride) {
+  for (long long first = (long long)blockIdx.x * kGroups; first < a.rows; first += (long long)gridDim.x * kGroups) {
     const long long row = first + group;
     const bool live = row < a.rows;
     const long long base = row * a.C;
-    const float rs = s;
-    float dot = 0.0f;
-    float nv[NV][VE], g[NV][VE];  // n and w dy
+    Pack<T, VE> ph[NV], py[NV], pd[NV];
+    const float s = live ? a.rstd_in[row] : 0.0f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int c = (n * LANES + lane) * VE;
-      const bool in = live && c < a.C;
+      if (!live || c >= a.C) continue;
+      ph[n] = *reinterpret_cast<const Pack<T, VE>*>(hp + base + c);
+      if (dy) py[n] = *reinterpret_cast<const Pack<T, VE>*>(dy + base + c);
+      if (dh) pd[n] = *reinterpret_cast<const Pack<T, VE>*>(dh + base + c);
+    }
+    float dot = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = (n * LANES + lane) * VE;
+      if (!live || c >= a.C || !dy) continue;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        nv[n][e] = in ? to_float(ph[n].v[e]) * rs : 0.0f;
-        const float d = in && dy ? to_float(py[n].v[e]) : 0.0f;
-        dw[n][e] = fmaf(d, nv[n][e], dw[n][e]);
-        g[n][e] = in && w ? d * to_float(pw[n].v[e]) : d;
-        dot = fmaf(g[n][e], nv[n][e], dot);
+        const float d = to_float(py[n].v[e]), nv = to_float(ph[n].v[e]) * s;
+        dw[n][e] = fmaf(d, nv, dw[n][e]);
+        dot = fmaf(w ? d * to_float(pw[n].v[e]) : d, nv, dot);
       }
     }
-    Pack<T, VE> up[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) up[n] = pd[n];
-    fetch(row + stride);
     if (!a.dx) continue;  // uniform
     dot = group_reduce<LANES, false>(dot, red) / (float)a.C;
 #pragma unroll
@@ -243,8 +230,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(const __grid_co
       if (!live || c >= a.C) continue;
       Pack<T, VE> po;
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        po.v[e] = from_float<T>(fmaf(rs, fmaf(-nv[n][e], dot, g[n][e]), dh ? to_float(up[n].v[e]) : 0.0f));
+      for (int e = 0; e < VE; ++e) {
+        const float d = dy ? to_float(py[n].v[e]) : 0.0f, nv = to_float(ph[n].v[e]) * s;
+        const float g = w ? d * to_float(pw[n].v[e]) : d;
+        po.v[e] = from_float<T>(fmaf(s, fmaf(-nv, dot, g), dh ? to_float(pd[n].v[e]) : 0.0f));
+      }
       *reinterpret_cast<Pack<T, VE>*>(reinterpret_cast<T*>(a.dx) + base + c) = po;
     }
   }
