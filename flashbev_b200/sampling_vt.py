@@ -17,12 +17,15 @@ tools/profile_differences.py:237 rely on.
                             381-447): project every voxel, keep the samples a camera sees, sort them
                             by BEV cell, pool each cell's interval with ``sampling_vt_pillarpool_fused``.
                             A comparison method too.
+  attention_heads=n      -> any of the above, followed by a block in which every BEV cell attends to the tokens of all
+                            cameras (``CameraAttention``); 0, the default, is the reference's module.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
 
+from .camera_attention import CameraAttention
 from .flash_bevpool import flash_bevpool
 from .sampling_vt_ops import sampling_vt_pillarpool_fused
 
@@ -146,7 +149,7 @@ class SamplingVT(nn.Module):
     def __init__(self, grid_config, input_size, downsample=16, in_channels=512, out_channels=64,
                  fuse_projection=True, use_bev_pool=True, use_shared_memory=False, fuse_bilinear=False,
                  depth_distribution="laplace", optimize_z_precompute=True, use_warp_kernel=False,
-                 use_vectorized_load=False, depth_weight_threshold=0.0):
+                 use_vectorized_load=False, depth_weight_threshold=0.0, attention_heads=0):
         super().__init__()
         self.use_bev_pool = use_bev_pool
         self.out_channels = out_channels
@@ -179,6 +182,12 @@ class SamplingVT(nn.Module):
             self.register_buffer("voxel_size", torch.as_tensor([a[2] for a in axes]))
             centres = [torch.linspace(a[0], a[1], g + 1)[:-1] + a[2] / 2.0 for a, g in zip(axes, self._grid)]
             self.register_buffer("coords_3d", torch.stack(torch.meshgrid(*centres, indexing="ij"), dim=-1))
+        self.camera_attention = None
+        if attention_heads:
+            # centres of the output cells (y, x) in metres
+            x, y = (a[0] + a[2] * (torch.arange(n, dtype=torch.float32) + 0.5) for a, n in zip(axes[:2], self._grid))
+            cells = torch.stack(torch.meshgrid(y, x, indexing="ij"), dim=-1).view(-1, 2)
+            self.camera_attention = CameraAttention(out_channels, out_channels, attention_heads, cells)
         # small constant inputs of the operator, built once per (device, B, N, h, w)
         self._const_cache = {}
 
@@ -211,7 +220,10 @@ class SamplingVT(nn.Module):
         features_pv = self._pointwise_conv(self.context_network, x)
         depths = self.forward_depth(x)
         # [B,C,Y,X] with channels-last strides: a channels-last BEV encoder consumes it without a copy
-        return self.sampling_vt(input, features_pv, depths), depths
+        bev = self.sampling_vt(input, features_pv, depths)
+        if self.camera_attention is not None:
+            bev = self.camera_attention(bev, features_pv, N)
+        return bev, depths
 
     def _constants(self, device, B, N, h, w):
         key = (str(device), B, N, h, w)

@@ -102,3 +102,17 @@ def test_rotary_and_norm_status_codes():
     assert grad(h=None) == 1 and grad(ws=None) == 8 and grad(n=8) == 8 and grad(ws=4100) == 8
     assert grad(gx=None, gw=None) == 0
     assert lib.fbev_add_rms_norm_grad_workspace_bytes(4, 16, 1) == 256 and lib.fbev_add_rms_norm_grad_workspace_bytes(4, 16, 0) == 0
+
+
+def test_camera_attention_is_optional_and_checks_its_sizes():
+    from flashbev_b200 import CameraAttention, SamplingVT
+    grid = {"x": [-4.0, 4.0, 1.0], "y": [-2.0, 2.0, 1.0], "z": [-4.0, 2.0, 1.0], "depth": [1.0, 60.0, 1.0]}
+    plain = SamplingVT(grid, (128, 352), in_channels=8, out_channels=16)
+    assert plain.camera_attention is None and not any("attention" in k for k in plain.state_dict())
+    m = SamplingVT(grid, (128, 352), in_channels=8, out_channels=16, attention_heads=2)
+    cells = m.camera_attention.cell_positions
+    assert cells.shape == (4 * 8, 2) and cells[0].tolist() == [-1.5, -3.5] and cells[-1].tolist() == [1.5, 3.5]
+    assert set(plain.state_dict()) < set(m.state_dict())
+    for channels, heads, key_heads in ((16, 3, None), (6, 2, None), (256, 1, None), (16, 4, 3), (16, 0, None)):
+        with pytest.raises(ValueError):
+            CameraAttention(channels, 8, heads, torch.zeros(4, 2), key_heads=key_heads)
