@@ -70,56 +70,62 @@ def _remember(plans: dict, key, plan):
     return plan
 
 
-def _operand(t: torch.Tensor, shared_batch: bool = False) -> torch.Tensor:
-    """``t`` [B,L,H,D] itself when the kernels can address it, else a contiguous copy.  They take any strides that are
-    multiples of 16 bytes, with the head's elements side by side; a view that repeats elements is copied, except along
-    a ``shared_batch``."""
-    per16 = 16 // t.element_size()
+def _taken(t: torch.Tensor, shared_batch: bool = False) -> bool:
+    """Whether the kernels take the strides of ``t`` [B,L,H,D] as they are.  A head's elements have to lie side by side.
+    16-bit heads of whole 16 bytes are fetched by the copy engine, which wants strides of whole 16 bytes and, except along
+    a ``shared_batch``, no repeated elements; everything else is read element by element, whatever the strides."""
     st, size = t.stride(), t.shape
-    good = (st[3] == 1 or size[3] == 1) and t.data_ptr() % 16 == 0
-    for i in range(3):
-        if size[i] > 1 and not (i == 0 and shared_batch):
-            good = good and st[i] > 0 and st[i] % per16 == 0
-    return t if good else t.clone(memory_format=torch.contiguous_format)
+    if st[3] != 1 and size[3] != 1:
+        return False
+    if t.element_size() != 2 or size[3] % 8:
+        return True
+    return all(st[i] > 0 and st[i] % 8 == 0 for i in range(3) if size[i] > 1 and not (i == 0 and shared_batch))
+
+
+def _operand(t: torch.Tensor, shared_batch: bool = False) -> torch.Tensor:
+    """``t`` itself when the kernels take it, else a contiguous copy."""
+    aligned = t.data_ptr() % 16 == 0 or t.element_size() != 2 or t.shape[3] % 8 != 0
+    return t if aligned and _taken(t, shared_batch) else t.clone(memory_format=torch.contiguous_format)
 
 
 class _AttentionPlan:
-    __slots__ = ("template", "workspace", "lse_count", "index")
+    __slots__ = ("template", "workspace", "lse_count", "index", "direct")
 
 
 _attention_plans: dict = {}
 
 
 def _attention_plan(q, k, v, lengths, mask, scale) -> _AttentionPlan:
-    """Of operands that _operand has been through."""
-    key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), q.dtype, q.device, lengths is None,
-           None if mask is None else mask.stride(0), scale)
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
+           v.device, lengths is None, None if mask is None else mask.stride(0), scale)
     plan = _attention_plans.get(key)
     if plan is not None:
         return plan
-    p = _lib.FbevAttention()
-    p.struct_size = ctypes.sizeof(_lib.FbevAttention)
-    p.dtype = _DTYPES[q.dtype]
-    p.B, p.Lq, p.Hq, p.D = q.shape
-    p.Lk, p.Hkv = k.shape[1], k.shape[2]
-    p.scale = scale
-    p.q_shared = 1 if p.B > 1 and q.stride(0) == 0 else 0
-    p.q_stride[:] = q.stride()[:3]
-    p.k_stride[:] = k.stride()[:3]
-    p.v_stride[:] = v.stride()[:3]
-    p.mask_stride = 0 if mask is None or p.B == 1 else mask.stride(0)
-    p.status = status_word(q.device).data_ptr()
-    # sizes depend on the addresses' alignment, which _operand has seen to, and on whether there are lengths
-    p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    if lengths is not None:
-        p.key_lengths = lengths.data_ptr()
-    lib = _lib.load()
+    _check_attention(q, k, v)
     plan = _AttentionPlan()
-    plan.workspace = tuple(lib.fbev_cross_attention_workspace_bytes(ctypes.byref(p), i) for i in (0, 1))
-    plan.lse_count = lib.fbev_cross_attention_lse_count(ctypes.byref(p))
+    plan.direct = _taken(q, shared_batch=True) and _taken(k) and _taken(v)
     plan.index = q.device.index
-    p.q = p.k = p.v = p.key_lengths = None
-    plan.template = bytes(p)
+    if plan.direct:
+        p = _lib.FbevAttention()
+        p.struct_size = ctypes.sizeof(_lib.FbevAttention)
+        p.dtype = _DTYPES[q.dtype]
+        p.B, p.Lq, p.Hq, p.D = q.shape
+        p.Lk, p.Hkv = k.shape[1], k.shape[2]
+        p.scale = 1.0 / math.sqrt(p.D) if scale is None else scale
+        p.q_shared = 1 if p.B > 1 and q.stride(0) == 0 else 0
+        p.q_stride[:] = q.stride()[:3]
+        p.k_stride[:] = k.stride()[:3]
+        p.v_stride[:] = v.stride()[:3]
+        p.mask_stride = 0 if mask is None or p.B == 1 else mask.stride(0)
+        p.status = status_word(q.device).data_ptr()
+        # the sizes follow from aligned addresses, which every call sees to, and from whether there are lengths
+        p.q = p.k = p.v = 4096
+        p.key_lengths = None if lengths is None else 4096
+        lib = _lib.load()
+        plan.workspace = tuple(lib.fbev_cross_attention_workspace_bytes(ctypes.byref(p), i) for i in (0, 1))
+        plan.lse_count = lib.fbev_cross_attention_lse_count(ctypes.byref(p))
+        p.q = p.k = p.v = p.key_lengths = None
+        plan.template = bytes(p)
     return _remember(_attention_plans, key, plan)
 
 
@@ -134,17 +140,16 @@ def _attention_problem(plan, q, k, v, lengths, mask, backward):
     nbytes = plan.workspace[backward]
     if not nbytes:
         return p, None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
     return p, ws
 
 
-def _attention_forward(q, k, v, lengths, mask, scale, with_lse):
-    plan = _attention_plan(q, k, v, lengths, mask, scale)
+def _attention_forward(plan, q, k, v, lengths, mask, with_lse):
     with _on(plan.index):
         p, ws = _attention_problem(plan, q, k, v, lengths, mask, 0)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(plan.lse_count, dtype=torch.float32, device=q.device) if with_lse else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = q.new_empty(plan.lse_count, dtype=torch.float32) if with_lse else None
         rc = _lib.load().fbev_cross_attention(ctypes.byref(p), out.data_ptr(), None if lse is None else lse.data_ptr(),
                                               _stream(plan.index))
     if rc:
@@ -154,8 +159,8 @@ def _attention_forward(q, k, v, lengths, mask, scale, with_lse):
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lengths, mask, scale):
-        out, lse = _attention_forward(q, k, v, lengths, mask, scale, True)
+    def forward(ctx, q, k, v, lengths, mask, scale, plan):
+        out, lse = _attention_forward(plan, q, k, v, lengths, mask, True)
         ctx.save_for_backward(q, k, v, lengths, mask, out, lse)
         ctx.scale = scale
         return out
@@ -164,9 +169,10 @@ class _CrossAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         q, k, v, lengths, mask, out, lse = ctx.saved_tensors
-        dev = q.device
         need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         gq = gk = gv = None
+        # saved tensors may come back at other addresses or strides (a hook moved them)
+        q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
         plan = _attention_plan(q, k, v, lengths, mask, ctx.scale)
         with _on(plan.index):
             go = grad_out.contiguous()
@@ -174,16 +180,16 @@ class _CrossAttention(torch.autograd.Function):
                 go = go.clone()
             p, ws = _attention_problem(plan, q, k, v, lengths, mask, 1)
             if need_q:
-                gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+                gq = torch.empty_like(q, memory_format=torch.contiguous_format)
             if need_kv:
-                gk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-                gv = torch.empty(v.shape, dtype=v.dtype, device=dev)
+                gk = torch.empty_like(k, memory_format=torch.contiguous_format)
+                gv = torch.empty_like(v, memory_format=torch.contiguous_format)
             rc = _lib.load().fbev_cross_attention_grad(
                 ctypes.byref(p), out.data_ptr(), lse.data_ptr(), go.data_ptr(), gq.data_ptr() if need_q else None,
                 gk.data_ptr() if need_kv else None, gv.data_ptr() if need_kv else None, _stream(plan.index))
         if rc:
             _lib.check(rc, "fbev_cross_attention_grad")
-        return (gq, gk if ctx.needs_input_grad[1] else None, gv if ctx.needs_input_grad[2] else None, None, None, None)
+        return gq, gk if ctx.needs_input_grad[1] else None, gv if ctx.needs_input_grad[2] else None, None, None, None, None
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_lengths: Optional[torch.Tensor] = None,
@@ -206,23 +212,20 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     type before they meet the values, as are the score gradients before they meet queries and keys.  Gradients are the
     same from run to run.  With few queries the keys are split over the GPU and the parts joined.
     """
-    # the checks pass once per combination of shapes, types and devices
-    key = (q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype, q.device, k.device, v.device)
-    if key not in _attention_checked:
-        _check_attention(q, k, v)
-        _remember(_attention_checked, key, True)
+    if scale is not None:
+        scale = float(scale)
+        if not math.isfinite(scale):
+            raise ValueError("scale must be finite")
     if key_lengths is not None or key_mask is not None:
+        _check_attention(q, k, v)
         key_lengths, key_mask = _attention_masks(q, k, key_lengths, key_mask)
-    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-    q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
+    plan = _attention_plan(q, k, v, key_lengths, key_mask, scale)
+    if not plan.direct or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
+        plan = _attention_plan(q, k, v, key_lengths, key_mask, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CrossAttention.apply(q, k, v, key_lengths, key_mask, scale)
-    return _attention_forward(q, k, v, key_lengths, key_mask, scale, False)[0]
-
-
-_attention_checked: dict = {}
+        return _CrossAttention.apply(q, k, v, key_lengths, key_mask, scale, plan)
+    return _attention_forward(plan, q, k, v, key_lengths, key_mask, False)[0]
 
 
 def _check_attention(q, k, v) -> None:
@@ -289,7 +292,7 @@ def _rotary(x, positions, sections, base, interleaved, inverse):
     p = _lib.FbevRotary.from_buffer_copy(template)
     p.x, p.positions = x.data_ptr(), positions.data_ptr()
     index = x.device.index
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     with _on(index):
         rc = _lib.load().fbev_rotary_axes(ctypes.byref(p), out.data_ptr(), _stream(index))
     if rc:
@@ -385,7 +388,7 @@ def _norm_forward(x, residual, weight, eps, with_rstd):
     index = x.device.index
     y = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if with_rstd else None
+    rstd = x.new_empty(rows, dtype=torch.float32) if with_rstd else None
     with _on(index):
         rc = _lib.load().fbev_add_rms_norm(_DTYPES[x.dtype], rows, C, eps, x.data_ptr(), _ptr(residual), _ptr(weight),
                                            y.data_ptr(), _ptr(h), _ptr(rstd), _stream(index))
@@ -420,7 +423,7 @@ class _AddRmsNorm(torch.autograd.Function):
             gx = torch.empty_like(h) if need_x else None
             gw = torch.empty_like(weight) if need_w else None
             nbytes = lib.fbev_add_rms_norm_grad_workspace_bytes(rows, C, int(need_w))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            ws = h.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
             rc = lib.fbev_add_rms_norm_grad(_DTYPES[h.dtype], rows, C, h.data_ptr(), rstd.data_ptr(), _ptr(weight),
                                             grad_y.data_ptr(), _ptr(grad_h), _ptr(gx), _ptr(gw), _ptr(ws), nbytes,
                                             _stream(dev.index))
@@ -461,8 +464,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
         lib = _lib.load()
         C = x.shape[-1]
         dev = x.device
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+        scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
         h = torch.empty_like(x) if residual is not None else None
         with _on(dev.index):
             rc = lib.fbev_add_rms_norm_e4m3(_DTYPES[x.dtype], x.numel() // C, C, eps, x.data_ptr(), _ptr(residual), _ptr(weight),
