@@ -20,7 +20,10 @@
 // and dP of the next; while they form dS, acc1 and S of the next.  All warps are in the same phase of a tile, so it is their
 // number that hides the latencies of a phase.
 //
-// Tensor memory, columns: S/P 0, dP/dS 128, acc0 256, acc1 384.
+// Where tensor memory has the room dP has two tiles in turn: with one, dP of the next tile waits for acc0 of this one, that
+// for dS, and dS for dP, and this round trip is the length of a step.
+//
+// Tensor memory, columns: S/P 0, dP/dS 128 (and 256), acc0 384 (or 256), acc1 448 (or 384).
 #pragma once
 #include "fbev_attention_tc.cuh"
 #include "fbev_rotary.cuh"
@@ -60,8 +63,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   using Shape = AttGradShape<NSUB>;
   constexpr int kStages = Shape::kStages;
   constexpr uint32_t kStageBytes = Shape::kStageBytes;
+  constexpr bool kTwo = NSUB == 1 || !KV;  // tiles of dP
+  constexpr uint32_t kAcc0 = kTwo ? 384 : 256, kAcc1 = NSUB == 1 ? 448 : 384;
   extern __shared__ unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t s_bar[3 * kStages + 7 + 2 * kMaskRing];
+  __shared__ __align__(8) uint64_t s_bar[3 * kStages + 9 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
   __shared__ __align__(16) float s_stat[KV ? kMaskRing : 1][2][128];  // -lse and -delta of the row tiles ahead
   __shared__ uint32_t s_tmem;
@@ -88,10 +93,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
   const auto fixed = [&](int s) { return bars + 8 * (2 * kStages + s); };
-  const uint32_t x_full = bars + 8 * (3 * kStages), s_full = x_full + 8, p_done = x_full + 16, dp_full = x_full + 24,
-                 ds_done = x_full + 32, acc_full = x_full + 40, drained = x_full + 48;
-  const auto m_full = [&](int i) { return drained + 8 + 8 * i; };
-  const auto m_empty = [&](int i) { return drained + 8 + 8 * (kMaskRing + i); };
+  const uint32_t x_full = bars + 8 * (3 * kStages), s_full = x_full + 8, p_done = x_full + 16, acc_full = x_full + 24, drained = x_full + 32;
+  // two barriers in turn where one of the sides may be a tile further than the other thinks: a barrier tells only its last
+  // phase from the one before
+  const auto dp_full = [&](int t) { return x_full + 40 + 8 * (t & 1); };
+  const auto ds_done = [&](int t) { return x_full + 56 + 8 * (t & 1); };
+  const auto dp_at = [&](int t) { return 128u + (kTwo ? 128u * (t & 1) : 0u); };
+  const auto m_full = [&](int i) { return x_full + 72 + 8 * i; };
+  const auto m_empty = [&](int i) { return x_full + 72 + 8 * (kMaskRing + i); };
 
   // dQ: keys that may not be attended are cleared before they meet dS, by a warp that follows the ring (as in the forward)
   const bool fixes = !KV && (masked || keys < a.p.Lk);
@@ -104,8 +113,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     mbar_init(x_full, 1);
     mbar_init(s_full, 1);
     mbar_init(p_done, 16);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_done, 16);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(dp_full(i), 1);
+      mbar_init(ds_done(i), 16);
+    }
     mbar_init(acc_full, 1);
     mbar_init(drained, 1);
     for (int i = 0; i < kMaskRing; ++i) {
@@ -209,8 +220,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       const auto dprobs = [&](int t) {
         wait_full(2 * t + 1);
         tc_fence_after();
-        product(tmem + 128, s_x + kStageBytes, stage(2 * t + 1), i_dp);
-        umma_commit(dp_full);
+        product(tmem + dp_at(t), s_x + kStageBytes, stage(2 * t + 1), i_dp);
+        umma_commit(dp_full(t));
         if (!KV) umma_commit(empty((2 * t + 1) % kStages));
       };
       scores(0);
@@ -219,15 +230,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         warp_wait(p_done, t & 1, bail);
         if (KV) {
           tc_fence_after();
-          accumulate(tmem + 384, tmem, stage(2 * t + 1), t == 0);
+          accumulate(tmem + kAcc1, tmem, stage(2 * t + 1), t == 0);
           umma_commit(empty((2 * t + 1) % kStages));
         }
-        if (t + 1 < n) scores(t + 1);
-        warp_wait(ds_done, t & 1, bail);
+        if (t + 1 < n) {
+          scores(t + 1);
+          if (kTwo) dprobs(t + 1);
+        }
+        warp_wait(ds_done(t), (t >> 1) & 1, bail);
         tc_fence_after();
-        accumulate(tmem + 256, tmem + 128, stage(2 * t), t == 0);
+        accumulate(tmem + kAcc0, tmem + dp_at(t), stage(2 * t), t == 0);
         umma_commit(empty((2 * t) % kStages));
-        if (t + 1 < n) dprobs(t + 1);
+        if (!kTwo && t + 1 < n) dprobs(t + 1);
       }
       umma_commit(acc_full);
       if (__any_sync(kFull, *bail.flag != 0)) {
@@ -295,7 +309,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     set_registers_up<104>();
     const int h = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = lanes + 32 * h, t_dp = lanes + 128 + 32 * h;
+    const uint32_t t_s = lanes + 32 * h;
     const long long row = (long long)xt * tile_rows + r;             // dQ
     const bool row_live = !KV && r < tile_rows && row < rows;
     const int key = xt * 128 + r;                                    // dK, dV
@@ -303,6 +317,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     const float nd = KV ? 0.0f : a.ndelta[((long long)bg * pl.row_tiles + xt) * 128 + r];
     for (int t = 0; t < n; ++t) {
       const int mr = t % kMaskRing;
+      const uint32_t t_dp = lanes + dp_at(t) + 32 * h;
       uint32_t word = kFull;
       if (!KV && masked) {
         warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
@@ -363,7 +378,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
 #pragma unroll
         for (int x = 0; x < 8; ++x) col[x] = *reinterpret_cast<const float4*>(&s_stat[mr][1][32 * h + 4 * x]);
       }
-      warp_wait(dp_full, t & 1, bail);
+      warp_wait(dp_full(t), (t >> 1) & 1, bail);
       tc_fence_after();
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
@@ -394,7 +409,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(ds_done);
+        mbar_arrive(ds_done(t));
         if (KV) mbar_arrive(m_empty(mr));
       }
     }
@@ -419,7 +434,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     for (int x = KV ? 32 * (h >> 1) : 32 * h; x < d16; x += KV ? 64 : 128) {
       float o[32];
       if (n > 0) {
-        tmem_ld32(lanes + (second ? 384 : 256) + x, o);
+        tmem_ld32(lanes + (second ? kAcc1 : kAcc0) + x, o);
         tmem_wait_ld();
       }
       if (zero) {
