@@ -14,16 +14,21 @@
 // S and dP are formed twice that way, seven products instead of the least of five; in exchange nothing of dQ travels to
 // memory in float32 and the result is the same from run to run.
 //
+// In the transposed kernel lse and delta belong to the columns.  Reading them by every thread, from shared memory that the
+// matrix instructions keep busy, took a third of a step.  They enter through the tensor cores instead: a 16-wide step more,
+// ones times three bfloat16 parts of -lse / c (24 bits, whatever the operands' type), leaves S - lse / c in the accumulator, and another dP - delta.  The
+// tile with the parts (columns 0 .. 2 and 16 .. 18) holds the ones too (columns 32 .. 34 of its rows).
+//
 // A 128 x 128 tile of S is in the hands of sixteen warps, a thread has 32 columns of a row: tensor memory -> registers ->
 // P in 16 bits back over S (needed as an operand only for dV), then dP -> dS in 16 bits back over dP.  Each quarter of the
 // columns writes over its own quarter only.  While the warps form P of the next tile, the tensor cores run acc0 of this one
 // and dP of the next; while they form dS, acc1 and S of the next.  All warps are in the same phase of a tile, so it is their
 // number that hides the latencies of a phase.
 //
-// Where tensor memory has the room dP has two tiles in turn: with one, dP of the next tile waits for acc0 of this one, that
+// For dQ, where tensor memory has the room, dP has two tiles in turn: with one, dP of the next tile waits for acc0 of this one, that
 // for dS, and dS for dP, and this round trip is the length of a step.
 //
-// Tensor memory, columns: S/P 0, dP/dS 128 (and 256), acc0 384 (or 256), acc1 448 (or 384).
+// Tensor memory, columns: S/P 0, dP/dS 128 (and 256), acc0 384; transposed: S/P 0, dP/dS 128, acc0 256, acc1 384.
 #pragma once
 #include "fbev_attention_tc.cuh"
 #include "fbev_rotary.cuh"
@@ -36,11 +41,11 @@ struct AttGradPlan {
 };
 
 struct AttGradArgs {
-  CUtensorMap x0, x1, y0, y1;
+  CUtensorMap x0, x1, y0, y1, z;
   FbevAttention p;
   AttGradPlan pl;
-  const float* nlse;    // -lse and -delta of every row, laid out by row tile: [B * Hkv][row_tiles][128], rows that are not
-  const float* ndelta;  // there have a weight of zero (-infinity) and no delta
+  const float* nlse;    // dQ: -lse and -delta of every row, laid out by row tile: [B * Hkv][row_tiles][128], rows that are
+  const float* ndelta;  // not there have a weight of zero (-infinity) and no delta; transposed: the same in the tiles of z
   void* g0;      // dQ, or dK
   void* g1;      // dV
   float* part0;  // float32 parts of g0 and g1 with splits > 1, unscaled
@@ -55,7 +60,7 @@ template <int NSUB>
 struct AttGradShape {
   static constexpr int kStages = NSUB == 1 ? 10 : 4;
   static constexpr uint32_t kStageBytes = NSUB * kTileBytes;
-  static constexpr uint32_t kSmem = (2 + kStages) * kStageBytes + 1024;
+  static constexpr uint32_t kSmem = (2 + kStages) * kStageBytes + 2 * kTileBytes + 1024;  // and two tiles of statistics
 };
 
 template <typename T, int NSUB, bool KV>
@@ -63,12 +68,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   using Shape = AttGradShape<NSUB>;
   constexpr int kStages = Shape::kStages;
   constexpr uint32_t kStageBytes = Shape::kStageBytes;
-  constexpr bool kTwo = NSUB == 1 || !KV;  // tiles of dP
-  constexpr uint32_t kAcc0 = kTwo ? 384 : 256, kAcc1 = NSUB == 1 ? 448 : 384;
+  constexpr bool kTwo = !KV;  // tiles of dP
+  constexpr uint32_t kAcc0 = kTwo ? 384 : 256, kAcc1 = 384;
   extern __shared__ unsigned char s_raw[];
   __shared__ __align__(8) uint64_t s_bar[3 * kStages + 9 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
-  __shared__ __align__(16) float s_stat[KV ? kMaskRing : 1][2][128];  // -lse and -delta of the row tiles ahead
   __shared__ uint32_t s_tmem;
   __shared__ int s_bail;
 
@@ -88,7 +92,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   n = n < 0 ? 0 : n > pl.per_split ? pl.per_split : n;
 
   const uint32_t smem = (smem_addr(s_raw) + 1023) & ~1023u;
-  const uint32_t s_x = smem, s_ring = smem + 2 * kStageBytes;
+  const uint32_t s_x = smem, s_ring = smem + 2 * kStageBytes,
+                 s_z = s_ring + kStages * kStageBytes;
   const uint32_t bars = smem_addr(s_bar);
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
@@ -121,7 +126,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     mbar_init(drained, 1);
     for (int i = 0; i < kMaskRing; ++i) {
       mbar_init(m_full(i), 1);
-      mbar_init(m_empty(i), 16);
+      mbar_init(m_empty(i), KV ? 1 : 16);
     }
     s_bail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -176,12 +181,20 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       };
       for (int t = 0; t < n; ++t) {
         load(&a.y0, t, qb);
+        if (KV) {  // the statistics' two tiles, by the mask ring's barriers
+          const int i = t & 1;
+          if (t >= 2) warp_wait(m_empty(i), ((t >> 1) - 1) & 1, bail);
+          mbar_expect(m_full(i), kTileBytes);
+          tma_load_4d(s_z + i * kTileBytes, &a.z, m_full(i), 0, 0, (t0 + t) * 128, bg);
+        }
         load(&a.y1, t, b);
       }
       if (__any_sync(kFull, *bail.flag != 0)) {
         // nothing may be left in flight when the block ends
         mbar_drain(x_full, 0);
         for (int i = slot > kStages ? slot - kStages : 0; i < slot; ++i) mbar_drain(full(i % kStages), (i / kStages) & 1);
+        if (KV)
+          for (int t = n > 2 ? n - 2 : 0; t < n; ++t) mbar_drain(m_full(t & 1), (t >> 1) & 1);
       }
     } else if (warp == 17 && n > 0) {
       // ---- matrix instructions -----------------------------------------------------------------------------------
@@ -206,8 +219,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
 #pragma unroll
         for (int k = 0; k < 8; ++k) umma_ts(d, t + 32 * (k / 2) + 8 * (k & 1), db + 128 * k, i_acc, !first || k > 0);
       };
+      const auto add_stat = [&](uint32_t d, int t, int at) {  // ones times the parts in columns at .. at + 15
+        const uint64_t z = desc_k_major(s_z + (t & 1) * kTileBytes);
+        umma_ss(d, z + 4, z + at / 8, umma_instr<__nv_bfloat16>(128, false, false), true);
+      };
       const auto scores = [&](int t) {
         wait_full(2 * t);
+        if (KV) warp_wait(m_full(t & 1), (t >> 1) & 1, bail);
         if (needs_fix(t)) {
           const int s = (2 * t) % kStages;
           warp_wait(fixed(s), (fix_parity >> s) & 1, bail);
@@ -215,13 +233,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         }
         tc_fence_after();
         product(tmem, s_x, stage(2 * t), i_s);
+        if (KV) add_stat(tmem, t, 0);
         umma_commit(s_full);
       };
       const auto dprobs = [&](int t) {
         wait_full(2 * t + 1);
         tc_fence_after();
         product(tmem + dp_at(t), s_x + kStageBytes, stage(2 * t + 1), i_dp);
+        if (KV) add_stat(tmem + dp_at(t), t, 16);
         umma_commit(dp_full(t));
+        if (KV) umma_commit(m_empty(t & 1));
         if (!KV) umma_commit(empty((2 * t + 1) % kStages));
       };
       scores(0);
@@ -290,19 +311,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         warp_wait(full(s1), ((2 * t + 1) / kStages) & 1, bail);
         release(s1);
       }
-    } else if (KV && warp == 18 && n > 0) {
-      // ---- statistics of the row tiles -----------------------------------------------------------------------------
-      const float4* nlse = reinterpret_cast<const float4*>(a.nlse + ((long long)bg * pl.row_tiles + t0) * 128);
-      const float4* ndelta = reinterpret_cast<const float4*>(a.ndelta + ((long long)bg * pl.row_tiles + t0) * 128);
-      for (int t = 0; t < n; ++t) {
-        const int m = t % kMaskRing;
-        const float4 l = nlse[32 * t + lane], d = ndelta[32 * t + lane];
-        if (t >= kMaskRing) warp_wait(m_empty(m), ((t / kMaskRing) - 1) & 1, bail);
-        *reinterpret_cast<float4*>(&s_stat[m][0][4 * lane]) = l;
-        *reinterpret_cast<float4*>(&s_stat[m][1][4 * lane]) = d;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(m_full(m));
-      }
     }
   } else {
     // ---- P and dS ----------------------------------------------------------------------------------------------------
@@ -328,13 +336,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         const int have = keys - (t0 + t) * 128 - 32 * h;
         word = have >= 32 ? kFull : have <= 0 ? 0u : (1u << have) - 1u;
       }
-      // the columns' statistics: read before the wait, while the tensor cores leave shared memory some room
-      float4 col[KV ? 8 : 1];
-      if (KV) {
-        warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) col[x] = *reinterpret_cast<const float4*>(&s_stat[mr][0][32 * h + 4 * x]);
-      }
       warp_wait(s_full, t & 1, bail);
       tc_fence_after();
       float p[32];
@@ -349,12 +350,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       for (int x = 0; x < 32; x += 16) {
         float2 e[8];
 #pragma unroll
-        for (int y = 0; y < 8; y += 2) {
-          const float* q = p + x + 2 * y;
-          float4 l = make_float4(nl, nl, nl, nl);
-          if (KV) l = col[(x + 2 * y) / 4];
-          e[y] = fma2(make_float2(q[0], q[1]), make_float2(a.c, a.c), make_float2(l.x, l.y));
-          e[y + 1] = fma2(make_float2(q[2], q[3]), make_float2(a.c, a.c), make_float2(l.z, l.w));
+        for (int y = 0; y < 8; ++y) {
+          const float2 s2 = make_float2(p[x + 2 * y], p[x + 2 * y + 1]), c2 = make_float2(a.c, a.c);
+          e[y] = KV ? mul2(s2, c2) : fma2(s2, c2, make_float2(nl, nl));
         }
         exp2_run<FBEV_POLY_GRAD>(e);
 #pragma unroll
@@ -374,10 +372,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(p_done);
       }
-      if (KV) {
-#pragma unroll
-        for (int x = 0; x < 8; ++x) col[x] = *reinterpret_cast<const float4*>(&s_stat[mr][1][32 * h + 4 * x]);
-      }
       warp_wait(dp_full(t), (t >> 1) & 1, bail);
       tc_fence_after();
 #pragma unroll
@@ -387,11 +381,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         tmem_wait_ld();
 #pragma unroll
         for (int x = 0; x < 16; x += 4) {
-          float4 d = make_float4(nd, nd, nd, nd);
-          if (KV) d = col[4 * y + x / 4];
           const float* q = p + 16 * y + x;
-          float2 s0 = mul2(add2(make_float2(dp[x], dp[x + 1]), make_float2(d.x, d.y)), make_float2(q[0], q[1]));
-          float2 s1 = mul2(add2(make_float2(dp[x + 2], dp[x + 3]), make_float2(d.z, d.w)), make_float2(q[2], q[3]));
+          float2 s0 = make_float2(dp[x], dp[x + 1]), s1 = make_float2(dp[x + 2], dp[x + 3]);
+          if (!KV) {
+            s0 = add2(s0, make_float2(nd, nd));
+            s1 = add2(s1, make_float2(nd, nd));
+          }
+          s0 = mul2(s0, make_float2(q[0], q[1]));
+          s1 = mul2(s1, make_float2(q[2], q[3]));
           if (word != kFull) {  // a select, not a product: what stands there may be NaN
             const uint32_t w = word >> (16 * y + x);
             if (!(w & 1)) s0.x = 0.0f;
@@ -408,10 +405,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(ds_done(t));
-        if (KV) mbar_arrive(m_empty(mr));
-      }
+      if (lane == 0) mbar_arrive(ds_done(t));
     }
     if (n > 0) warp_wait(acc_full, 0, bail);
     tc_fence_after();
@@ -476,7 +470,7 @@ constexpr int kStatRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ FbevAttention p, int TL, int row_tiles, const T* __restrict__ out,
                                                        const T* __restrict__ go, const float* __restrict__ lse, float* __restrict__ nlse,
-                                                       float* __restrict__ ndelta) {
+                                                       float* __restrict__ ndelta, uint4* __restrict__ parts, float inv_c) {
   const int lane = threadIdx.x & 7, G = p.Hq / p.Hkv;
   const unsigned rows = (unsigned)att_rows(p);
   // blocks of 128 rows: one row tile
@@ -495,7 +489,7 @@ __global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ F
         x[k][i] = *reinterpret_cast<const Pack<T, 8>*>(out + head + lane * 8 + 64 * i);
         y[k][i] = *reinterpret_cast<const Pack<T, 8>*>(go + head + lane * 8 + 64 * i);
       }
-    l[k] = live[k] && lane == 0 ? lse[bg * att_rows_padded(p) + row] : INFINITY;
+    l[k] = live[k] ? lse[bg * att_rows_padded(p) + row] : INFINITY;
   }
 #pragma unroll
   for (int k = 0; k < kStatRows; ++k) {
@@ -508,10 +502,28 @@ __global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ F
       }
 #pragma unroll
     for (int s = 4; s > 0; s >>= 1) d[k] += __shfl_xor_sync(kFull, d[k], s);
+    const long long at = (long long)blockIdx.x * 128 + 32 * k + (threadIdx.x >> 3);
     if (lane == 0) {
-      const long long at = (long long)blockIdx.x * 128 + 32 * k + (threadIdx.x >> 3);
       nlse[at] = -l[k];
       ndelta[at] = -d[k];
+    }
+    if (parts != nullptr) {
+      // lane i: columns 8 i .. 8 i + 7 of the row's 64
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (lane == 0 || lane == 2) {
+        float v = lane == 0 ? -l[k] * inv_c : -d[k];
+        const bool finite = fabsf(v) < 3.0e38f;
+        const uint32_t p0 = pack2<__nv_bfloat16>(v, 0.0f);
+        v = finite ? v - __uint_as_float(p0 << 16) : 0.0f;
+        const uint32_t p1 = pack2<__nv_bfloat16>(v, 0.0f);
+        v = finite ? v - __uint_as_float(p1 << 16) : 0.0f;
+        w.x = p0 | p1 << 16;
+        w.y = pack2<__nv_bfloat16>(v, 0.0f);
+      } else if (lane == 4) {
+        w.x = pack2<__nv_bfloat16>(1.0f, 1.0f);
+        w.y = pack2<__nv_bfloat16>(1.0f, 0.0f);
+      }
+      parts[at * 8 + lane] = w;
     }
   }
   grid_dependency_trigger();

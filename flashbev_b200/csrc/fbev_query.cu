@@ -484,11 +484,14 @@ static size_t gradient_part_bytes(const FbevAttention& p, bool kv) {  // of one 
 static size_t stat_bytes(const FbevAttention& p) {  // -lse or -delta by row tile
   return (size_t)p.B * p.Hkv * gradient_plan(p, false).row_tiles * 512;
 }
-// both statistics, then the parts of dQ, and after those are summed the parts of dK and dV in the same place
+static size_t stat_tile_bytes(const FbevAttention& p) {  // and the tiles in which they meet the matrix instructions
+  return 32 * stat_bytes(p);
+}
+// both statistics, their tiles, then the parts of dQ, and after those are summed the parts of dK and dV in the same place
 static size_t backward_workspace(const FbevAttention& p) {
   if (!direct(p)) return split_layout(p, true).bytes;
   const size_t q = gradient_part_bytes(p, false), kv = 2 * gradient_part_bytes(p, true);
-  return 2 * stat_bytes(p) + (q > kv ? q : kv);
+  return 2 * stat_bytes(p) + stat_tile_bytes(p) + (q > kv ? q : kv);
 }
 
 template <typename T, int NSUB, bool KV>
@@ -506,12 +509,19 @@ static int tensor_gradient(const FbevAttention& p, const T* go, T* g0, T* g1, cu
   if (rc == FBEV_OK) rc = encode_rows(KV ? &a.y1 : &a.x1, p, rows, go, go_stride, false);
   if (rc == FBEV_OK) rc = encode_keys(KV ? &a.x0 : &a.y0, p, p.k, p.k_stride);
   if (rc == FBEV_OK) rc = encode_keys(KV ? &a.x1 : &a.y1, p, p.v, p.v_stride);
-  if (rc != FBEV_OK) return rc;
   char* ws = reinterpret_cast<char*>(p.workspace);
+  if (KV && rc == FBEV_OK) {
+    const long long rows = 128ll * a.pl.row_tiles, dims[4] = {64, 1, rows, (long long)p.B * p.Hkv}, strides[4] = {1, 64, 64, 64 * rows};
+    const int box[4] = {64, 1, 128, 1};
+    rc = encode_map(&a.z, p.dtype, 4, ws + 2 * stat_bytes(p), dims, strides, box);
+  } else {
+    a.z = a.x0;
+  }
+  if (rc != FBEV_OK) return rc;
   a.nlse = reinterpret_cast<const float*>(ws);
   a.ndelta = reinterpret_cast<const float*>(ws + stat_bytes(p));
-  a.part0 = reinterpret_cast<float*>(ws + 2 * stat_bytes(p));
-  a.part1 = reinterpret_cast<float*>(ws + 2 * stat_bytes(p) + gradient_part_bytes(p, KV));
+  a.part0 = reinterpret_cast<float*>(ws + 2 * stat_bytes(p) + stat_tile_bytes(p));
+  a.part1 = reinterpret_cast<float*>(ws + 2 * stat_bytes(p) + stat_tile_bytes(p) + gradient_part_bytes(p, KV));
   a.g0 = g0;
   a.g1 = g1;
   a.c = score_factor(p);
@@ -533,7 +543,8 @@ static int tensor_backward(const FbevAttention& p, const T* out, const float* ls
   float* nlse = reinterpret_cast<float*>(p.workspace);
   float* ndelta = reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + stat_bytes(p));
   const unsigned blocks = (unsigned)((long long)p.B * p.Hkv * pl.row_tiles);
-  att_stat_kernel<T><<<blocks, 256, 0, st>>>(p, pl.TL, pl.row_tiles, out, go, lse, nlse, ndelta);
+  uint4* tiles = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.workspace) + 2 * stat_bytes(p));
+  att_stat_kernel<T><<<blocks, 256, 0, st>>>(p, pl.TL, pl.row_tiles, out, go, lse, nlse, ndelta, gk ? tiles : nullptr, 1.0f / score_factor(p));
   int rc = cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
   if (rc == FBEV_OK && gq) rc = tensor_gradient<T, NSUB, false>(p, go, gq, (T*)nullptr, st);
   if (rc == FBEV_OK && gk) rc = tensor_gradient<T, NSUB, true>(p, go, gk, gv, st);
