@@ -466,21 +466,24 @@ __global__ void __launch_bounds__(256) att_sum_kernel(const float* __restrict__ 
 
 // -lse and -delta = -<out, grad_out> of every row of the padded row tiles: eight lanes share a row, 16 bytes a load, and have
 // kStatRows rows in flight
-constexpr int kStatRows = 4;
+constexpr int kStatRows = 2;
 template <typename T>
 __global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ FbevAttention p, int TL, int row_tiles, const T* __restrict__ out,
                                                        const T* __restrict__ go, const float* __restrict__ lse, float* __restrict__ nlse,
                                                        float* __restrict__ ndelta, uint4* __restrict__ parts, float inv_c) {
   const int lane = threadIdx.x & 7, G = p.Hq / p.Hkv;
   const unsigned rows = (unsigned)att_rows(p);
-  // blocks of 128 rows: one row tile
-  const unsigned bg = blockIdx.x / (unsigned)row_tiles, tile = blockIdx.x - bg * (unsigned)row_tiles, b = bg / p.Hkv, g = bg - b * p.Hkv;
+  // blocks of 32 * kStatRows rows of a row tile
+  constexpr unsigned kBlocks = 4 / kStatRows;
+  const unsigned all = blockIdx.x / kBlocks, part = blockIdx.x - all * kBlocks;
+  const unsigned bg = all / (unsigned)row_tiles, tile = all - bg * (unsigned)row_tiles, b = bg / p.Hkv, g = bg - b * p.Hkv;
+  const unsigned first = 32 * kStatRows * part + (threadIdx.x >> 3);
   float d[kStatRows], l[kStatRows];
   Pack<T, 8> x[kStatRows][2], y[kStatRows][2];
   bool live[kStatRows];
 #pragma unroll
   for (int k = 0; k < kStatRows; ++k) {
-    const unsigned r = 32 * k + (threadIdx.x >> 3), row = tile * TL * G + r, q = row / G;
+    const unsigned r = first + 32 * k, row = tile * TL * G + r, q = row / G;
     live[k] = r < (unsigned)(TL * G) && row < rows;
     const long long head = (((long long)b * p.Lq + q) * p.Hq + g * G + (row - q * G)) * p.D;
 #pragma unroll
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(256) att_stat_kernel(const __grid_constant__ F
       }
 #pragma unroll
     for (int s = 4; s > 0; s >>= 1) d[k] += __shfl_xor_sync(kFull, d[k], s);
-    const long long at = (long long)blockIdx.x * 128 + 32 * k + (threadIdx.x >> 3);
+    const long long at = (long long)all * 128 + first + 32 * k;
     if (lane == 0) {
       nlse[at] = -l[k];
       ndelta[at] = -d[k];

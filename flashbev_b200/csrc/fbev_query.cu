@@ -542,7 +542,7 @@ static int tensor_backward(const FbevAttention& p, const T* out, const float* ls
   const AttGradPlan pl = gradient_plan(p, false);
   float* nlse = reinterpret_cast<float*>(p.workspace);
   float* ndelta = reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + stat_bytes(p));
-  const unsigned blocks = (unsigned)((long long)p.B * p.Hkv * pl.row_tiles);
+  const unsigned blocks = (unsigned)((long long)p.B * p.Hkv * pl.row_tiles * (4 / kStatRows));
   uint4* tiles = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.workspace) + 2 * stat_bytes(p));
   att_stat_kernel<T><<<blocks, 256, 0, st>>>(p, pl.TL, pl.row_tiles, out, go, lse, nlse, ndelta, gk ? tiles : nullptr, 1.0f / score_factor(p));
   int rc = cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
