@@ -28,7 +28,10 @@
 // For dQ, where tensor memory has the room, dP has two tiles in turn: with one, dP of the next tile waits for acc0 of this one, that
 // for dS, and dS for dP, and this round trip is the length of a step.
 //
-// Tensor memory, columns: S/P 0, dP/dS 128 (and 256), acc0 384; transposed: S/P 0, dP/dS 128, acc0 256, acc1 384.
+// Transposed, with heads up to 64 wide, S has two tiles instead: the next one is formed before P of this one is used up.
+//
+// Tensor memory, columns: S/P 0, dP/dS 128 and 256, acc0 384; transposed: S/P 0 and 128, dP/dS 256, acc0 384, acc1 448, or
+// with wide heads S/P 0, dP/dS 128, acc0 256, acc1 384.
 #pragma once
 #include "fbev_attention_tc.cuh"
 #include "fbev_rotary.cuh"
@@ -68,10 +71,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   using Shape = AttGradShape<NSUB>;
   constexpr int kStages = Shape::kStages;
   constexpr uint32_t kStageBytes = Shape::kStageBytes;
-  constexpr bool kTwo = !KV;  // tiles of dP
-  constexpr uint32_t kAcc0 = kTwo ? 384 : 256, kAcc1 = 384;
+  constexpr bool kTwo = !KV;               // tiles of dP
+  constexpr bool kTwoS = KV && NSUB == 1;  // and of S
+  constexpr uint32_t kAcc0 = kTwo || kTwoS ? 384 : 256, kAcc1 = kTwoS ? 448 : 384;
   extern __shared__ unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t s_bar[3 * kStages + 9 + 2 * kMaskRing];
+  __shared__ __align__(8) uint64_t s_bar[3 * kStages + 11 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_bail;
@@ -98,14 +102,17 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
   const auto fixed = [&](int s) { return bars + 8 * (2 * kStages + s); };
-  const uint32_t x_full = bars + 8 * (3 * kStages), s_full = x_full + 8, p_done = x_full + 16, acc_full = x_full + 24, drained = x_full + 32;
+  const uint32_t x_full = bars + 8 * (3 * kStages), acc_full = x_full + 8, drained = x_full + 16;
   // two barriers in turn where one of the sides may be a tile further than the other thinks: a barrier tells only its last
   // phase from the one before
-  const auto dp_full = [&](int t) { return x_full + 40 + 8 * (t & 1); };
-  const auto ds_done = [&](int t) { return x_full + 56 + 8 * (t & 1); };
-  const auto dp_at = [&](int t) { return 128u + (kTwo ? 128u * (t & 1) : 0u); };
-  const auto m_full = [&](int i) { return x_full + 72 + 8 * i; };
-  const auto m_empty = [&](int i) { return x_full + 72 + 8 * (kMaskRing + i); };
+  const auto s_full = [&](int t) { return x_full + 24 + 8 * (t & 1); };
+  const auto p_done = [&](int t) { return x_full + 40 + 8 * (t & 1); };
+  const auto dp_full = [&](int t) { return x_full + 56 + 8 * (t & 1); };
+  const auto ds_done = [&](int t) { return x_full + 72 + 8 * (t & 1); };
+  const auto s_at = [&](int t) { return kTwoS ? 128u * (t & 1) : 0u; };
+  const auto dp_at = [&](int t) { return kTwo ? 128u + 128u * (t & 1) : kTwoS ? 256u : 128u; };
+  const auto m_full = [&](int i) { return x_full + 88 + 8 * i; };
+  const auto m_empty = [&](int i) { return x_full + 88 + 8 * (kMaskRing + i); };
 
   // dQ: keys that may not be attended are cleared before they meet dS, by a warp that follows the ring (as in the forward)
   const bool fixes = !KV && (masked || keys < a.p.Lk);
@@ -116,9 +123,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       mbar_init(fixed(s), 1);
     }
     mbar_init(x_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(p_done, 16);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full(i), 1);
+      mbar_init(p_done(i), 16);
       mbar_init(dp_full(i), 1);
       mbar_init(ds_done(i), 16);
     }
@@ -232,9 +239,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
           fix_parity ^= 1u << s;
         }
         tc_fence_after();
-        product(tmem, s_x, stage(2 * t), i_s);
-        if (KV) add_stat(tmem, t, 0);
-        umma_commit(s_full);
+        product(tmem + s_at(t), s_x, stage(2 * t), i_s);
+        if (KV) add_stat(tmem + s_at(t), t, 0);
+        umma_commit(s_full(t));
       };
       const auto dprobs = [&](int t) {
         wait_full(2 * t + 1);
@@ -248,13 +255,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       scores(0);
       dprobs(0);
       for (int t = 0; t < n; ++t) {
-        warp_wait(p_done, t & 1, bail);
+        if (kTwoS && t + 1 < n) scores(t + 1);
+        warp_wait(p_done(t), (t >> 1) & 1, bail);
         if (KV) {
           tc_fence_after();
-          accumulate(tmem + kAcc1, tmem, stage(2 * t + 1), t == 0);
+          accumulate(tmem + kAcc1, tmem + s_at(t), stage(2 * t + 1), t == 0);
           umma_commit(empty((2 * t + 1) % kStages));
         }
-        if (t + 1 < n) {
+        if (!kTwoS && t + 1 < n) {
           scores(t + 1);
           if (kTwo) dprobs(t + 1);
         }
@@ -317,7 +325,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     set_registers_up<104>();
     const int h = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = lanes + 32 * h;
     const long long row = (long long)xt * tile_rows + r;             // dQ
     const bool row_live = !KV && r < tile_rows && row < rows;
     const int key = xt * 128 + r;                                    // dK, dV
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
     const float nd = KV ? 0.0f : a.ndelta[((long long)bg * pl.row_tiles + xt) * 128 + r];
     for (int t = 0; t < n; ++t) {
       const int mr = t % kMaskRing;
-      const uint32_t t_dp = lanes + dp_at(t) + 32 * h;
+      const uint32_t t_s = lanes + s_at(t) + 32 * h, t_dp = lanes + dp_at(t) + 32 * h;
       uint32_t word = kFull;
       if (!KV && masked) {
         warp_wait(m_full(mr), (t / kMaskRing) & 1, bail);
@@ -336,7 +343,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         const int have = keys - (t0 + t) * 128 - 32 * h;
         word = have >= 32 ? kFull : have <= 0 ? 0u : (1u << have) - 1u;
       }
-      warp_wait(s_full, t & 1, bail);
+      warp_wait(s_full(t), (t >> 1) & 1, bail);
       tc_fence_after();
       float p[32];
       tmem_ld32(t_s, p);
@@ -344,7 +351,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
       if (!KV) {  // S may be overwritten
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_done);
+        if (lane == 0) mbar_arrive(p_done(t));
       }
 #pragma unroll
       for (int x = 0; x < 32; x += 16) {
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_done);
+        if (lane == 0) mbar_arrive(p_done(t));
       }
       warp_wait(dp_full(t), (t >> 1) & 1, bail);
       tc_fence_after();
