@@ -18,6 +18,7 @@ BWD_FEATS, BWD_DEPTH, BWD_LEGACY_DEPTH, BWD_DETERMINISTIC = 1, 2, 4, 8
 DEV_BAD_FEATURE_SIZE, DEV_TIMEOUT = 1, 2
 POS_F32, POS_I32, POS_I64 = 0, 1, 2
 ROTARY_MAX_PAIRS = 128
+ATTENTION_MAX_SCALE = 1e30
 WORKSPACE_BYTES = 16
 STATIC_SCRATCH_BYTES = 16 << 20
 SORT_BUDGET_BYTES = 256 << 20

@@ -23,6 +23,11 @@
 // leave normalised float32 outputs and their logarithmic sums for att_join_kernel.
 //
 // Tensor memory, columns: S/P tiles from 0 (128 each), O of the two groups behind them (64 or 128 each).
+//
+// Bound by the exponentials and what surrounds them in the softmax warps with heads of 64 (2 x 8100 queries x 5400 keys x 8
+// heads: 235 us, 750 TFLOP/s; the unit for exponentials alone would need 150 us), by the tensor cores with heads of 128
+// (2 x 8100 x 8448 x 8: 520 us, 1.09 PFLOP/s), by the memory's rate with one query a sample (64 samples, lengths up to
+// 16384: 150 us, 84 % of the copy rate).
 #pragma once
 #include "fbev_attention.cuh"
 #include "fbev_tc.cuh"
@@ -66,13 +71,11 @@ struct AttFwdShape {
 // the exponent.  The unit for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with
 // the rest of the softmax; a part of the weights goes this way instead.  What is below 2^-126 becomes 2^-126: a score of
 // -infinity leaves a weight that no sum notices, and rows without any key are told by their maximum.
-// this many of eight pairs
-#ifndef FBEV_POLY_FWD
-#define FBEV_POLY_FWD 1
-#endif
-#ifndef FBEV_POLY_GRAD
-#define FBEV_POLY_GRAD 3
-#endif
+//
+// How many of eight pairs: 0, 1, 2, 3, 4 gave 258, 244, 246, 248, 276 us in the forward at 2 x 8100 queries x 5400 keys x 8
+// heads of 64, and 522, 522, 526, 533, 555 us at 2 x 8100 x 8448 x 8 heads of 128.  In the gradients, whose threads have two
+// of the multiply-add pipe's long phases a tile to hide it in, 3 was the shortest.
+constexpr int kPolyForward = 1, kPolyGrad = 3;
 // eight pairs at once; the steps of the cubics side by side, the other exponentials between them
 template <int OF8>
 __device__ __forceinline__ void exp2_run(float2 (&x)[8]) {
@@ -489,7 +492,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
               const int z = 64 * half + 2 * (x + y);
               e[y] = fma2(make_float2(s[z], s[z + 1]), make_float2(a.c, a.c), make_float2(off, off));
             }
-            exp2_run<FBEV_POLY_FWD>(e);
+            exp2_run<kPolyForward>(e);
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
               part[y & 3] = add2(part[y & 3], e[y]);

@@ -1,5 +1,6 @@
-// The operators of include/fbev_query.h: argument checks, plans, launches and the C ABI.  Kernels:
-// fbev_attention.cuh, fbev_rotary.cuh, fbev_norm.cuh.
+// The operators of include/fbev_query.h: argument checks, plans, launches and the C ABI.  Kernels: fbev_attention_tc.cuh and
+// fbev_attention_grad_tc.cuh (16-bit attention and its gradients), fbev_attention_split_tc.cuh (float32, and what TMA cannot
+// address), fbev_rotary.cuh, fbev_norm.cuh.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,6 +28,7 @@ static int check_attention(const FbevAttention* p) {
   if (!known_dtype(p->dtype)) return FBEV_ERR_DTYPE;
   if (p->B < 0 || p->Lq < 0 || p->Lk < 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->D <= 0 || p->D > 128)
     return FBEV_ERR_SHAPE;
+  if (!(p->scale >= -1e30f && p->scale <= 1e30f)) return FBEV_ERR_RANGE;
   if (att_rows(*p) >= (1ll << 31) || (long long)p->B * p->Hq >= (1ll << 31)) return FBEV_ERR_RANGE;
   if ((long long)p->B * p->Hkv * (att_rows(*p) + 256) >= (1ll << 31) || (long long)p->B * p->Hkv * (p->Lk + 256ll) >= (1ll << 31))
     return FBEV_ERR_RANGE;  // blocks of a launch
@@ -93,7 +95,7 @@ static SplitChoice choose_splits(int units, int tiles, double part, bool ragged,
       best = {0, s, per};
     }
     if (tail && full > 0 && rest > 0) {
-      const double d = full / kSms * (tiles + 3) + waves((double)rest * s) * (per + 3) + (rest * s / (double)kSms) * part + 2;
+      const double d = (double)(full / kSms) * (tiles + 3) + waves((double)rest * s) * (per + 3) + (rest * s / (double)kSms) * part + 2;
       if (d < 0.98 * cost) {
         cost = d;
         best = {full, s, per};

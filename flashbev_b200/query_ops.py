@@ -203,19 +203,22 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
             slices of one projection's output), others are copied.
         key_lengths: [B] int32 or int64: only the first so many keys of a sample may be attended (clamped to 0..Lk).
         key_mask: [B,Lk] or [Lk] bool, True where a key may be attended.  Both may be given: both must allow.
-        scale: factor of the scores; default 1 / sqrt(D).
+        scale: factor of the scores; default 1 / sqrt(D).  At most 1e30 in magnitude.
     Returns:
         [B,Lq,Hq,D] in the dtype of q.  Rows that may attend nothing are zero, and so are their gradients.  What
         stands in keys and values that may not be attended (infinities, NaN) has no influence.
 
     Scores, softmax statistics and sums are float32; for 16-bit inputs the softmax weights are rounded to the input's
-    type before they meet the values, as are the score gradients before they meet queries and keys.  Gradients are the
-    same from run to run.  With few queries the keys are split over the GPU and the parts joined.
+    type before they meet the values, as are the score gradients before they meet queries and keys: in float16 those lose
+    what is below 2^-24 and overflow beyond 65504, so train with a scaled loss there, as with any float16 gradient.
+    float32 operands enter the products as three bfloat16 parts each, which keeps 24 bits; an infinity (or a value beyond
+    3.38e38) among float32 operands that are attended gives NaN.  Gradients are the same from run to run.  With few
+    queries the keys are split over the GPU and the parts joined.
     """
     if scale is not None:
         scale = float(scale)
-        if not math.isfinite(scale):
-            raise ValueError("scale must be finite")
+        if not abs(scale) <= _lib.ATTENTION_MAX_SCALE:
+            raise ValueError(f"scale must be finite and at most {_lib.ATTENTION_MAX_SCALE:g} in magnitude, got {scale}")
     if key_lengths is not None or key_mask is not None:
         _check_attention(q, k, v)
         key_lengths, key_mask = _attention_masks(q, k, key_lengths, key_mask)
@@ -436,7 +439,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
                  eps: float = 1e-6, quantize: bool = False):
     """Residual addition and root-mean-square norm over the last dimension.
 
-    ``h = x + residual``, ``y = h / sqrt(mean(h ** 2) + eps) * weight``, in float32 from the unrounded sum.
+    ``h = x + residual``, ``y = h / sqrt(mean(h ** 2) + eps) * weight``, in float32 from the unrounded sum (the squares of a
+    row have to stay within float32).
 
     Args:
         x: [..., C].  residual: the same shape, or None.  weight: [C], or None for ones.  All of one dtype.
@@ -453,7 +457,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
         _remember(_norm_checked, key, True)
     if not 0.0 <= eps < math.inf:
         raise ValueError("eps must be finite and not negative")
-    x = x.contiguous()
+    given, x = x, x.contiguous()
     residual = None if residual is None else residual.contiguous()
     weight = None if weight is None else weight.contiguous()
     grad = torch.is_grad_enabled() and (
@@ -472,12 +476,12 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
                                             q.data_ptr(), scales.data_ptr(), _ptr(h), _stream(dev.index))
         if rc:
             _lib.check(rc, "fbev_add_rms_norm_e4m3")
-        return q, scales, x if h is None else h
+        return q, scales, given if h is None else h
     if not grad:
         y, h, _ = _norm_forward(x, residual, weight, eps, False)
-        return y, x if h is None else h
+        return y, given if h is None else h
     if residual is None:
-        return _AddRmsNorm.apply(x, None, weight, eps), x
+        return _AddRmsNorm.apply(x, None, weight, eps), given
     return _AddRmsNorm.apply(x, residual, weight, eps)
 
 

@@ -32,7 +32,7 @@ typedef struct FbevAttention {
   int32_t dtype;              /* FBEV_F32 / FBEV_BF16 / FBEV_F16: q, k, v, the output and all gradients */
   int32_t B, Lq, Lk;          /* samples, queries, keys; zeros are allowed */
   int32_t Hq, Hkv, D;         /* query heads, key heads (a divisor of Hq), head width 1..128 */
-  float scale;
+  float scale;                /* finite, at most 1e30 in magnitude */
   int32_t q_shared;           /* 1: the queries are the same for every sample; q_stride[0] is not used */
   int64_t q_stride[3];        /* elements from sample to sample, token to token, head to head; the head's elements */
   int64_t k_stride[3];        /*   are contiguous */
@@ -49,19 +49,19 @@ typedef struct FbevAttention {
 } FbevAttention;
 
 /* Number of float32 values of the statistics tensor `lse`: one per query and head, each (sample, key head) padded to a
- * multiple of four; 0 for an invalid problem. */
+ * multiple of four; 0 for an invalid problem.  A forward with Lk = 0 leaves them as they were (its backward reads none). */
 size_t fbev_cross_attention_lse_count(const FbevAttention* p);
 
 /* Device bytes of workspace for the forward (backward = 0) or the backward (backward = 1); 0 for an invalid problem. */
 size_t fbev_cross_attention_workspace_bytes(const FbevAttention* p, int backward);
 
-/* out: device, contiguous [B,Lq,Hq,D], 16-byte aligned.  lse: device, 16-byte aligned, fbev_cross_attention_lse_count() floats for the
- * backward, or NULL. */
+/* out: device, contiguous [B,Lq,Hq,D], 16-byte aligned.  lse: device, 16-byte aligned, fbev_cross_attention_lse_count()
+ * floats for the backward, or NULL. */
 int fbev_cross_attention(const FbevAttention* p, void* out, float* lse, void* stream);
 
 /* Gradients of sum(out * grad_out).  out, grad_out: contiguous [B,Lq,Hq,D]; lse: as the forward left it.
- * grad_q [B,Lq,Hq,D], grad_k and grad_v [B,Lk,Hkv,D], contiguous, overwritten; all 16-byte aligned; grad_q, or grad_k and grad_v together,
- * may be NULL.  The results do not depend on the order in which blocks run. */
+ * grad_q [B,Lq,Hq,D], grad_k and grad_v [B,Lk,Hkv,D], contiguous, overwritten; all 16-byte aligned; grad_q, or grad_k and
+ * grad_v together, may be NULL.  The results do not depend on the order in which blocks run. */
 int fbev_cross_attention_grad(const FbevAttention* p, const void* out, const float* lse, const void* grad_out,
                               void* grad_q, void* grad_k, void* grad_v, void* stream);
 

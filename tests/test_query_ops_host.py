@@ -116,3 +116,12 @@ def test_camera_attention_is_optional_and_checks_its_sizes():
     for channels, heads, key_heads in ((16, 3, None), (6, 2, None), (256, 1, None), (16, 4, 3), (16, 0, None)):
         with pytest.raises(ValueError):
             CameraAttention(channels, 8, heads, torch.zeros(4, 2), key_heads=key_heads)
+
+
+def test_scores_have_a_finite_factor():
+    lib = _lib.load()
+    for scale in (float("nan"), float("inf"), -float("inf"), 2e30, -2e30):
+        p = _attention()
+        p.scale = scale
+        assert lib.fbev_cross_attention(ctypes.byref(p), 4096, None, None) == 7
+        assert lib.fbev_cross_attention_grad(ctypes.byref(p), 4096, 4096, 4096, 4096, 4096, 4096, None) == 7
