@@ -83,8 +83,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   extern __shared__ unsigned char s_raw[];
   __shared__ __align__(8) uint64_t s_bar[3 * kStages + 11 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
+  __shared__ uint8_t s_list[kSkipTiles];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_bail;
+  __shared__ int s_bail, s_count;
 
   const AttGradPlan& pl = a.pl;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -100,6 +101,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
   const int t0 = split * pl.per_split;
   int n = (KV ? (xt * 128 < keys ? pl.row_tiles : 0) : (keys + 127) / 128) - t0;  // tiles Y of this block
   n = n < 0 ? 0 : n > pl.per_split ? pl.per_split : n;
+  // dQ skips the tiles of keys that the mask empties; a block of dK and dV whose keys are all masked has nothing to do
+  const bool skips = masked && n > 0 && (KV || n <= kSkipTiles);
+  if (skips) {
+    const uint8_t* mask = a.p.key_mask + (long long)b * a.p.mask_stride;
+    const int left = uniform(att_tiles_left<kGradThreads / 32>(mask, keys, KV ? xt : t0, KV ? 1 : n, s_list, &s_count));
+    n = KV ? (left > 0 ? n : 0) : left;
+  }
+  const auto y_tile = [&](int t) { return t0 + (!KV && skips ? uniform(s_list[t]) : t); };
 
   const uint32_t smem = (smem_addr(s_raw) + 1023) & ~1023u;
   const uint32_t s_x = smem, s_ring = smem + 2 * kStageBytes,
@@ -189,7 +198,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         if (KV)
           load_rows(s_ring + s * kStageBytes, map, full(s), t0 + t, batch);
         else
-          load_keys(s_ring + s * kStageBytes, map, full(s), t0 + t);
+          load_keys(s_ring + s * kStageBytes, map, full(s), y_tile(t));
         ++slot;
       };
       for (int t = 0; t < n; ++t) {
@@ -296,7 +305,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) att_grad_kernel(const __grid_
         if (fix) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int j = (t0 + t) * 128 + 32 * i + lane;
+            const int j = y_tile(t) * 128 + 32 * i + lane;
             word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
           }
         }

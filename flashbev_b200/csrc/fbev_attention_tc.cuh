@@ -150,8 +150,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   __shared__ __align__(8) uint64_t s_bar[3 * kStages + 3 * kBufs + 6 + 2 * kMaskRing];
   __shared__ uint32_t s_mask[kMaskRing][4];
   __shared__ float s_stat[2][128];
+  __shared__ uint8_t s_list[kSkipTiles];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_bail;
+  __shared__ int s_bail, s_count;
 
   const AttPlan& pl = a.pl;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -171,6 +172,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   const bool pair = pl.pair != 0;
   const int tiles = pair ? 1 : (pl.row_tiles - 2 * rb < 2 ? 1 : 2);  // row tiles of this block
   const bool masked = a.p.key_mask != nullptr;
+  const bool skips = masked && n > 0 && n <= kSkipTiles;
+  if (skips) n = uniform(att_tiles_left<kAttThreads / 32>(a.p.key_mask + (long long)b * a.p.mask_stride, keys, t0, n, s_list, &s_count));
+  const auto key_tile = [&](int t) { return t0 + (skips ? uniform(s_list[t]) : t); };
   const long long rows = att_rows(a.p);
   const int tile_rows = pl.TL * pl.G;
 
@@ -250,8 +254,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         const int s = slot % kStages;
         if (slot >= kStages) warp_wait(empty(s), ((slot / kStages) - 1) & 1, bail);
         mbar_expect(full(s), kStageBytes);
+        const int tile = key_tile(t);
         for (int x = 0; x < NSUB; ++x)
-          tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, (t0 + t) * 128, b);
+          tma_load_4d(s_ring + s * kStageBytes + x * kTileBytes, map, full(s), 64 * x, g, tile * 128, b);
         ++slot;
       };
       for (int q = 0; q < kBufs && q < steps; ++q)
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
       };
       for (int q = 0; q < kBufs && q < steps; ++q)
         if (new_tile(q)) release(follow());
-      for (int q = 0; q < steps ; ++q) {
+      for (int q = 0; q < steps; ++q) {
         const bool keys_next = q + kBufs < steps && new_tile(q + kBufs);
         if (!new_tile(q)) {
           if (keys_next) {
@@ -372,7 +377,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         if (fix) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int j = (t0 + t) * 128 + 32 * i + lane;
+            const int j = key_tile(t) * 128 + 32 * i + lane;
             word[i] = __ballot_sync(kFull, j < keys && (!masked || mask[j] != 0));
           }
         }
