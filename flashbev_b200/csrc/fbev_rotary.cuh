@@ -164,7 +164,8 @@ static int rotary_launch(const FbevRotary* p, T* out, cudaStream_t st) {
   const auto fits = [&](int ve) {
     const int unit = p->interleaved ? 2 * p->pairs : p->pairs;
     bool ok = unit % ve == 0 && (p->D - 2 * p->pairs) % ve == 0 && p->D % ve == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && p->x_stride[i] % ve == 0;
+    const int size[3] = {p->B, p->L, p->H};  // the stride of a dimension of one is never used
+    for (int i = 0; i < 3; ++i) ok = ok && (size[i] == 1 || p->x_stride[i] % ve == 0);
     return ok && (uintptr_t)p->x % (ve * sizeof(T)) == 0 && (uintptr_t)out % (ve * sizeof(T)) == 0;
   };
   if (fits(kWide)) return rotary_launch_ve<T, P, kWide>(p, out, st);

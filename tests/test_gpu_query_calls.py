@@ -105,6 +105,16 @@ def test_norm_without_residual_returns_its_argument(cuda_device):
     assert add_rms_norm(x, quantize=True)[2] is x
 
 
+def test_strides_of_dimensions_of_one(cuda_device):
+    """A head cut out of an odd row: the strides of dimensions of one are odd, and not used."""
+    for dtype in (F32, BF16):
+        x, p = _rand((1, 1, 1, 17), dtype, 1)[..., :16], torch.full((1, 1), 3.0, device=cuda_device)
+        for inter in (False, True):
+            assert R.worst(rotary_axes(x, p, (8,), interleaved=inter), R.rotary(x, p, (8,), 10000.0, inter)) <= 1.0
+        k = _rand((1, 40, 1, 17), dtype, 2)[..., :16]
+        assert R.worst(cross_attention(x, k, k), R.attention(x, k, k, R.allowed(1, 40), 0.25)["out"]) <= 1.0
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
 def test_one_gradient_at_a_time(cuda_device, dtype):
     q, k, v = _rand((2, 200, 4, 64), dtype, 1), _rand((2, 900, 2, 64), dtype, 2), _rand((2, 900, 2, 64), dtype, 3)
