@@ -129,6 +129,15 @@ def _attention_plan(q, k, v, lengths, mask, scale) -> _AttentionPlan:
     return _remember(_attention_plans, key, plan)
 
 
+def _planned(q, k, v, lengths, mask, scale):
+    """The plan of a call and its operands, copied where the kernels do not take them as they are."""
+    plan = _attention_plan(q, k, v, lengths, mask, scale)
+    if not plan.direct or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
+        plan = _attention_plan(q, k, v, lengths, mask, scale)
+    return plan, q, k, v
+
+
 def _attention_problem(plan, q, k, v, lengths, mask, backward):
     """The filled struct and the workspace, which has to live until the launch is queued."""
     p = _lib.FbevAttention.from_buffer_copy(plan.template)
@@ -172,8 +181,7 @@ class _CrossAttention(torch.autograd.Function):
         need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         gq = gk = gv = None
         # saved tensors may come back at other addresses or strides (a hook moved them)
-        q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
-        plan = _attention_plan(q, k, v, lengths, mask, ctx.scale)
+        plan, q, k, v = _planned(q, k, v, lengths, mask, ctx.scale)
         with _on(plan.index):
             go = grad_out.contiguous()
             if go.data_ptr() % 16:
@@ -220,12 +228,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
         if not abs(scale) <= _lib.ATTENTION_MAX_SCALE:
             raise ValueError(f"scale must be finite and at most {_lib.ATTENTION_MAX_SCALE:g} in magnitude, got {scale}")
     if key_lengths is not None or key_mask is not None:
-        _check_attention(q, k, v)
+        if k.dim() != 4:
+            _check_attention(q, k, v)
         key_lengths, key_mask = _attention_masks(q, k, key_lengths, key_mask)
-    plan = _attention_plan(q, k, v, key_lengths, key_mask, scale)
-    if not plan.direct or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
-        q, k, v = _operand(q, shared_batch=True), _operand(k), _operand(v)
-        plan = _attention_plan(q, k, v, key_lengths, key_mask, scale)
+    plan, q, k, v = _planned(q, k, v, key_lengths, key_mask, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossAttention.apply(q, k, v, key_lengths, key_mask, scale, plan)
     return _attention_forward(plan, q, k, v, key_lengths, key_mask, False)[0]
@@ -250,11 +256,13 @@ def _attention_masks(q, k, key_lengths, key_mask):
             raise ValueError(f"key_lengths must be int32 or int64 of shape [{B}]")
         if key_lengths.dtype == torch.int64:
             key_lengths = key_lengths.clamp(0, Lk)
-        key_lengths = key_lengths.to(device=q.device, dtype=torch.int32).contiguous()
+        if key_lengths.dtype != torch.int32 or key_lengths.device != q.device or not key_lengths.is_contiguous():
+            key_lengths = key_lengths.to(device=q.device, dtype=torch.int32).contiguous()
     if key_mask is not None:
         if key_mask.dtype != torch.bool or key_mask.shape not in ((B, Lk), (Lk,)):
             raise ValueError(f"key_mask must be bool of shape [{B},{Lk}] or [{Lk}]")
-        key_mask = key_mask.to(q.device)
+        if key_mask.device != q.device:
+            key_mask = key_mask.to(q.device)
         if key_mask.dim() == 1:
             key_mask = key_mask.unsqueeze(0).expand(B, Lk)
         if Lk > 1 and key_mask.stride(1) != 1:
