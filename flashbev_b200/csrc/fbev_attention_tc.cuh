@@ -186,7 +186,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
   const auto fixed = [&](int s) { return bars + 8 * (2 * kStages + s); };
   const uint32_t q_full = bars + 8 * (3 * kStages), drained = q_full + 8;
   const auto o_full = [&](int i) { return q_full + 16 + 8 * i; };  // the group's last product is done
-  const auto o_step = [&](int i) { return q_full + 32 + 8 * i; };  // ... each one
+  // the product of each step, by two barriers in turn.  A barrier tells only its last phase from the one before: who waits for
+  // the step before its own has to know of the product two phases back.  The scores it holds came after the product kBufs
+  // steps ago, and two steps are one phase.
+  const auto o_step = [&](int q) { return q_full + 32 + 8 * (q & 1); };
   const auto s_full = [&](int i) { return q_full + 48 + 8 * i; };
   const auto p_half = [&](int i) { return q_full + 48 + 8 * (kBufs + i); };
   const auto p_full = [&](int i) { return q_full + 48 + 8 * (2 * kBufs + i); };
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         warp_wait(p_full(buf), parity, bail);
         if (!Shape::kHalves) values(q, sv, 0, q < streams);
         values(q, sv, 1, false);
-        umma_commit(o_step(i));
+        umma_commit(o_step(q));
         if (q + streams >= steps) umma_commit(o_full(i));
         if (last_use(q)) umma_commit(empty(sv));
         if (more) {
@@ -466,11 +469,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           const float back = raise ? (m == -INFINITY ? 0.0f : exp2_fast(m - mt)) : 1.0f;
           if (raise) m = mt;
           sum *= back;
-          // the output so far has to be complete.  A barrier tells only its last phase from the one before, so the product
-          // before the last one has to be known as done: with two streams it came before these scores, with one it is waited for.
+          // the output so far has to be complete
           if (j > 0) {
-            if (streams == 1 && j > 1) warp_wait(o_step(i), j & 1, bail);
-            warp_wait(o_step(i), (j - 1) & 1, bail);
+            const int last = q - streams;
+            warp_wait(o_step(last), (last >> 1) & 1, bail);
             tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < d16; x += 32) {

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from flashbev_b200 import add_rms_norm, cross_attention, rotary_axes
+from flashbev_b200.flash_bevpool import status_word
 from tests import query_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -267,3 +268,24 @@ def test_more_masked_tiles_than_a_block_lists(cuda_device):
         one = slice(b, b + 1)
         want = R.attention(q[one], k[one], k[one], R.allowed(1, Lk, None, mask[one]), 0.125, None)
         assert R.worst(out[one], want["out"]) <= 1.0, b
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Lq", [1, 100, 128, 129, 300, 640])
+def test_maximum_that_rises_late(cuda_device, Lq, D, dtype):
+    """Every number of row tiles a block may have, with scores that rise along the keys, so that the output so far is
+    rescaled in late tiles, and with first tiles that are masked."""
+    Lk = 1100
+    q, k, v = _rand((1, Lq, 2, D), dtype, 1), _rand((1, Lk, 2, D), dtype, 2), _rand((1, Lk, 2, D), dtype, 3)
+    k = (k.float() * torch.linspace(0.05, 6, Lk, device=cuda_device).view(1, Lk, 1, 1)).to(dtype)
+    q, dout = (q.float() * 4).to(dtype), _rand(q.shape, dtype, 4)
+    for first in (0, 1, 200, 520):
+        mask = torch.arange(Lk, device=cuda_device) >= first
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = cross_attention(*leaves, key_mask=mask)
+        want = R.attention(q, k, v, R.allowed(1, Lk, None, mask), 1 / math.sqrt(D), dout)
+        assert R.worst(out, want["out"]) <= 1.0, first
+        for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout)):
+            assert R.worst(got, want[name]) <= 1.0, (first, name)
+    assert int(status_word(torch.device("cuda", 0)).item()) & 2 == 0
