@@ -382,6 +382,7 @@ struct SplitSource {
   long long stride[3];
   int G;                    // heads folded into rows
   int L, shared;
+  int whole;                // rows and strides of whole fours of elements at such addresses
   __nv_bfloat16* parts;     // [B * Hkv][L * G][3][width]
   int width;                // D rounded up to eight
   float* allowed;           // keys: [B][tiles][128], and the rows of keys that may not be attended are zeros
@@ -397,59 +398,76 @@ struct SplitSet {
   unsigned first[5];  // blocks of each
 };
 
-// The parts of all tensors in one launch: a warp per row, four elements a lane.  Bound by memory: 4 bytes in, 6 out per
-// element.
-template <typename T>
+// The parts of all tensors in one launch: LANES (16, or 32 for heads above 64) a row, four elements a lane.  Bound by
+// memory: 4 bytes in, 6 out per element.  Both directions of 2 x 32109 rows of 64: 34 us, 65 with a warp for each row, whole
+// divisions of 64 bits and loads of single elements.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ FbevAttention p, const __grid_constant__ SplitSet set) {
   int which = 0;
   while (blockIdx.x >= set.first[which + 1]) ++which;
   const SplitSource& s = set.of[which];
-  const long long rows = (long long)s.L * s.G, tiles = (rows + 127) / 128,
-                  unit = (long long)(blockIdx.x - set.first[which]) * 8 + (threadIdx.x >> 5);
-  const long long bg = unit / (tiles * 128), row = unit - bg * tiles * 128;
-  const int lane = threadIdx.x & 31, D = p.D;
+  // all below 2^31; whole divisions of 64 bits would be most of the kernel
+  const unsigned rows = (unsigned)s.L * (unsigned)s.G, tiles = (rows + 127) / 128,
+                 unit = (blockIdx.x - set.first[which]) * (256 / LANES) + threadIdx.x / LANES;
+  const unsigned tile = unit >> 7, bg = tile / tiles, row = unit - bg * tiles * 128;
+  const int lane = threadIdx.x % LANES, D = p.D;
   grid_dependency_trigger();
-  if (bg >= (long long)p.B * p.Hkv) return;
-  const long long b = bg / p.Hkv, l = row / s.G;
+  const unsigned b = bg / (unsigned)p.Hkv, l = row / (unsigned)s.G;
   const int g = (int)(bg - b * p.Hkv), h = g * s.G + (int)(row - l * s.G);
   bool there = row < rows;
+  bool clear = false;
   if (s.allowed != nullptr) {
-    const bool may = there && row < att_keys(p, (int)b) && att_allowed(p, (int)b, (int)row);
-    if (g == 0 && lane == 0) s.allowed[b * tiles * 128 + row] = may ? 0.0f : -INFINITY;
-    if (there && !may) {
-      if (4 * lane < s.width)
-        for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(s.parts + ((bg * rows + row) * 3 + i) * s.width + 4 * lane) = make_uint2(0, 0);
-      there = false;
-    }
+    const bool may = there && (int)row < att_keys(p, (int)b) && att_allowed(p, (int)b, (int)row);
+    if (g == 0 && lane == 0) s.allowed[(long long)b * tiles * 128 + row] = may ? 0.0f : -INFINITY;
+    clear = there && !may;
+    there = may;
   }
+  const bool mine = 4 * lane < s.width;
+  Pack<T, 4> v, o;
   float x[4] = {};
-  if (there) {
-    const T* src = reinterpret_cast<const T*>(s.src) + (s.shared ? 0 : b * s.stride[0]) + l * s.stride[1] + h * s.stride[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * lane + i < D) x[i] = to_float(src[4 * lane + i]);
-  }
-  if (s.nlse != nullptr) {
-    float d = 0.0f;
-    if (there) {
-      const T* out = reinterpret_cast<const T*>(s.out) + ((b * p.Lq + l) * p.Hq + h) * D;
+  const bool dots = s.nlse != nullptr;
+  if (there && mine) {
+    const T* src = reinterpret_cast<const T*>(s.src) + (s.shared ? 0 : b * s.stride[0]) + l * s.stride[1] + h * s.stride[2] + 4 * lane;
+    const T* out = reinterpret_cast<const T*>(s.out) + (((long long)b * p.Lq + l) * p.Hq + h) * D + 4 * lane;
+    if (s.whole) {  // four elements at once
+      if (4 * lane < D) {
+        v = *reinterpret_cast<const Pack<T, 4>*>(src);
+        if (dots) o = *reinterpret_cast<const Pack<T, 4>*>(out);
+      }
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (4 * lane + i < D) d = fmaf(x[i], to_float(out[4 * lane + i]), d);
+        if (4 * lane + i < D) {
+          v.v[i] = src[i];
+          if (dots) o.v[i] = out[i];
+        }
     }
-    d = warp_sum(d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * lane + i < D) x[i] = to_float(v.v[i]);
+  }
+  if (dots) {
+    float d = 0.0f;
+    if (there && mine) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * lane + i < D) d = fmaf(x[i], to_float(o.v[i]), d);
+    }
+#pragma unroll
+    for (int k = LANES / 2; k > 0; k >>= 1) d += __shfl_xor_sync(kFull, d, k);
     if (lane == 0) {
       s.nlse[unit] = there ? -s.lse[bg * att_rows_padded(p) + row] : -INFINITY;
       s.ndelta[unit] = -d;
     }
   }
-  if (!there || 4 * lane >= s.width) return;
+  if (!(there || clear) || !mine) return;
+  __nv_bfloat16* parts = s.parts + ((long long)bg * rows + row) * 3 * s.width + 4 * lane;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 3; ++i) {  // zeros where a key is cleared
     uint2 w;
     w.x = pack2<__nv_bfloat16>(x[0], x[1]);
     w.y = pack2<__nv_bfloat16>(x[2], x[3]);
-    *reinterpret_cast<uint2*>(s.parts + ((bg * rows + row) * 3 + i) * s.width + 4 * lane) = w;
+    *reinterpret_cast<uint2*>(parts + i * s.width) = w;
     x[0] -= __uint_as_float(w.x << 16);
     x[1] -= __uint_as_float(w.x & 0xffff0000u);
     x[2] -= __uint_as_float(w.y << 16);

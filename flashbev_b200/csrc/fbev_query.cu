@@ -313,6 +313,8 @@ static int split_operands(const FbevAttention& p, const SplitLayout& l, const T*
     s.G = g;
     s.L = len;
     s.shared = shared;
+    s.whole = p.D % 4 == 0 && (uintptr_t)src % (4 * sizeof(T)) == 0;
+    for (int k = 0; k < 3; ++k) s.whole = s.whole && stride[k] % 4 == 0;
     s.parts = reinterpret_cast<__nv_bfloat16*>(ws + at);
     s.width = l.width;
   };
@@ -333,11 +335,14 @@ static int split_operands(const FbevAttention& p, const SplitLayout& l, const T*
   long long blocks = 0;
   for (int i = 0; i < 4; ++i) {
     set.first[i] = (unsigned)blocks;
-    if (i < count) blocks += (long long)p.B * p.Hkv * (((long long)set.of[i].L * set.of[i].G + 127) / 128) * 16;
+    if (i < count) blocks += (long long)p.B * p.Hkv * (((long long)set.of[i].L * set.of[i].G + 127) / 128) * (p.D <= 64 ? 8 : 16);
     if (blocks >= (1ll << 31)) return FBEV_ERR_RANGE;
     set.first[i + 1] = (unsigned)blocks;
   }
-  split_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(p, set);
+  if (p.D <= 64)
+    split_kernel<T, 16><<<(unsigned)blocks, 256, 0, st>>>(p, set);
+  else
+    split_kernel<T, 32><<<(unsigned)blocks, 256, 0, st>>>(p, set);
   return cudaGetLastError() == cudaSuccess ? FBEV_OK : FBEV_ERR_LAUNCH;
 }
 
