@@ -67,8 +67,8 @@ struct AttFwdShape {
 };
 
 // 2^x of two numbers on the multiply-add pipe, for weights that are rounded to 16 bits: x = n + f with n whole and
-// |f| <= 1/2, 2^f by the cubic with the least largest relative error on that interval (2^-13.7, Remez exchange), n added to
-// the exponent.  The unit for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with
+// |f| <= 1/2, 2^f by the cubic with the least largest relative error on that interval (2^-13.7, Remez exchange), times 2^n,
+// whose bits the rounding of x leaves in place: a product, not an addition to the exponent, so that NaN stays NaN.  The unit for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with
 // the rest of the softmax; a part of the weights goes this way instead.  What is below 2^-126 becomes 2^-126: a score of
 // -infinity leaves a weight that no sum notices, and rows without any key are told by their maximum.
 //
@@ -91,12 +91,12 @@ __device__ __forceinline__ void exp2_run(float2 (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < OF8; ++i) {
     x[i] = make_float2(max_nan(x[i].x, -126.0f), max_nan(x[i].y, -126.0f));
-    r[i] = add2(x[i], make_float2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: the whole part in the low bits
+    r[i] = add2(x[i], make_float2(12583039.0f, 12583039.0f));  // 1.5 * 2^23 + 127: n + 127 in the low bits
   }
   between(1);
 #pragma unroll
   for (int i = 0; i < OF8; ++i) {
-    const float2 n = add2(r[i], make_float2(-12582912.0f, -12582912.0f));
+    const float2 n = add2(r[i], make_float2(-12583039.0f, -12583039.0f));
     f[i] = fma2(n, make_float2(-1.0f, -1.0f), x[i]);
   }
   between(2);
@@ -111,8 +111,7 @@ __device__ __forceinline__ void exp2_run(float2 (&x)[8]) {
   between(5);
 #pragma unroll
   for (int i = 0; i < OF8; ++i)
-    x[i] = make_float2(__uint_as_float((__float_as_uint(r[i].x) << 23) + __float_as_uint(p[i].x)),
-                       __uint_as_float((__float_as_uint(r[i].y) << 23) + __float_as_uint(p[i].y)));
+    x[i] = mul2(p[i], make_float2(__uint_as_float(__float_as_uint(r[i].x) << 23), __uint_as_float(__float_as_uint(r[i].y) << 23)));
 }
 
 constexpr int kMaskRing = 4;
