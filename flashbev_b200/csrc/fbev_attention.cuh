@@ -2,7 +2,8 @@
 //
 // Rows.  The G = Hq / Hkv query heads that share a key head are folded into rows: row r of (sample, key head) is query
 // r / G, head r % G of the group.  Statistics are laid out by row: lse[(b * Hkv + g) * rows_padded + r] =
-// log2 sum_j 2^(S_j log2 e), +infinity for a row without keys, so that 2^(S - lse) is zero there.
+// log2 sum_j 2^(S_j log2 e), +infinity for a row without keys, so that 2^(S - lse) is zero there, NaN for a row whose scores
+// are not numbers or all -infinity.
 #pragma once
 #include "fbev_device.cuh"
 #include "fbev_query.h"
@@ -10,6 +11,7 @@
 namespace fbev {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;  // statistic of a part whose keys all score -infinity
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

@@ -328,13 +328,25 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       sum = s_max[0][0][r];
-      f = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     const bool parted = a.part != nullptr;
+    bool lost = false;                                  // no score above -infinity though there are keys (as in fbev_attention_tc.cuh)
+    bool none = MODE == kSplitDq && nl == -INFINITY;    // no keys; scores that are not numbers are NaN at masked keys too
+    if (MODE == kSplitOut) {
+      if (__any_sync(kFull, !(sum > 0.0f))) {
+        bool seen = false;
+        for (int j = lane; j < 128 * n; j += 32) seen = seen || col[j] == 0.0f;
+        seen = __any_sync(kFull, seen);
+        none = !seen;
+        lost = seen && sum == 0.0f;
+      }
+      if (none) sum = 0.0f;
+      f = lost && !parted ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+    }
     if (kDs && parted) f = 1.0f;  // the scale is applied to the sum of the parts
     if (live) {
       const int G = a.p.Hq / a.p.Hkv;
-      bool zero = n == 0;
+      bool zero = n == 0 || none;
       if (kKeyRows) zero = zero || a.allowed[((long long)b * key_tiles + xt) * 128 + r] != 0.0f;
       const long long heads = (long long)a.p.B * a.p.Hkv;
       const long long at = kKeyRows ? (((long long)b * a.p.Lk + row) * a.p.Hkv + g) * a.p.D
@@ -363,8 +375,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_split_kernel(const __grid_
       }
       if (MODE == kSplitOut && h == 0) {
         const long long padded = att_rows_padded(a.p);
-        if (parted) a.part_lse[(split * heads + bg) * a.x_tiles * 128 + row] = sum == 0.0f ? -INFINITY : m + log2f(sum);
-        else if (a.lse != nullptr) a.lse[bg * padded + row] = sum == 0.0f ? INFINITY : m + log2f(sum);
+        if (parted) a.part_lse[(split * heads + bg) * a.x_tiles * 128 + row] = lost ? kLowest : sum == 0.0f ? -INFINITY : m + log2f(sum);
+        else if (a.lse != nullptr) a.lse[bg * padded + row] = lost ? NAN : sum == 0.0f ? INFINITY : m + log2f(sum);
       }
     }
     tc_fence_before();

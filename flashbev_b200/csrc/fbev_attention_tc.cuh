@@ -14,6 +14,10 @@
 // up to 64 wide tensor memory holds three score tiles, so a group finds its next one ready; with two it waits for both
 // products.
 //
+// NaN scores do not raise the maximum, they show in the sum, from where they reach the output and the statistics.  A row whose
+// keys all score -infinity has the statistic kLowest instead of the -infinity of a row without keys: its output is NaN, as a
+// quotient of zeros, while the latter's is zero; of several parts of a row only those above it count.
+//
 // m is the row's running maximum, raised only when a tile exceeds it by more than 8: weights then stay below 2^8 (no loss
 // in either type, both sides of the quotient carry the same factor) and the output, which lives in tensor memory, is
 // rescaled in a few of the first tiles only.
@@ -425,6 +429,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
     const bool live = works && r < tile_rows && row < rows;
     const int d16 = (a.p.D + 15) / 16 * 16;
     float m = -INFINITY, sum = 0.0f;
+    bool seen = mine > 0 && !masked;  // a key that may be attended (the same for all rows)
     if (works) {
       for (int j = 0; j < mine; ++j) {
         const int q = j * streams + i, t = tile_of(q), buf = q % kBufs;
@@ -439,6 +444,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
           __syncwarp();
           if (lane == 0) mbar_arrive(m_empty(mr));
           cut = (word[0] & word[1] & word[2] & word[3]) != kFull;
+          seen = seen || (word[0] | word[1] | word[2] | word[3]) != 0;
         } else if ((t0 + t + 1) * 128 > keys) {
           const int have = keys - (t0 + t) * 128;
 #pragma unroll
@@ -520,6 +526,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(buf));
       }
+      if (seen && m == -INFINITY) {  // scores, but none above -infinity
+        m = kLowest;
+        sum = sum * 0.0f + 1.0f;     // NaN stays
+      }
       if (mine > 0) warp_wait(o_full(i), 0, bail);
       // the second group is about to write over the ring: the first group's tiles must have been consumed too
       if (pair && i == 1 && mine > 0) warp_wait(o_full(0), 0, bail);
@@ -555,7 +565,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) att_fwd_kernel(const __grid_co
         sum = sum * f0 + sum1 * f1;
         m = mm;
       }
-      const bool none = m == -INFINITY;  // no key
+      const bool none = m == -INFINITY;             // no key
+      if (m == kLowest && !parted) sum = NAN;  // parts: the join tells whether another one has a score
       const float inv = none ? 0.0f : 1.0f / sum;
       const long long l = row / pl.G;
       T* dst = reinterpret_cast<T*>(a.out) + (((long long)b * a.p.Lq + l) * a.p.Hq + g * pl.G + (int)(row - l * pl.G)) * a.p.D;
@@ -616,7 +627,8 @@ struct JoinArgs {
   int warps;              // warps that share a row: 4 or 1
 };
 
-// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s.  Few rows: a block per row, whose warps take
+// out[row] = sum over splits of 2^(lse_s - L) o_s with L = log2 sum_s 2^lse_s; NaN where a part is, and where no part has a
+// score above -infinity though one has keys.  Few rows: a block per row, whose warps take
 // the splits in turn (in a fixed order) and add up in shared memory; many: a warp per row.
 template <typename T>
 __global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ FbevAttention p, const __grid_constant__ JoinArgs a, T* __restrict__ out) {
@@ -631,11 +643,12 @@ __global__ void __launch_bounds__(128) att_join_kernel(const __grid_constant__ F
   if (slot % 128 >= a.tile_rows || row >= rows) return;  // the whole block where it shares a row
   const long long step = (long long)a.units * a.slots, at = (long long)u * a.slots + slot;
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_lse[s * step + at]);
+  for (int s = lane; s < a.splits; s += 32) top = max_nan(top, a.part_lse[s * step + at]);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-  float total = 0.0f, o[4] = {};
-  if (top != -INFINITY) {
+  for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, d));
+  const bool scored = top > kLowest;  // not with NaN
+  float total = scored || top == -INFINITY ? 0.0f : NAN, o[4] = {};
+  if (scored) {
 #pragma unroll 4
     for (int s = a.warps == 4 ? warp : 0; s < a.splits; s += a.warps) {
       const float w = exp2_fast(a.part_lse[s * step + at] - top);

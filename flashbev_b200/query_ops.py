@@ -214,13 +214,15 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
         scale: factor of the scores; default 1 / sqrt(D).  At most 1e30 in magnitude.
     Returns:
         [B,Lq,Hq,D] in the dtype of q.  Rows that may attend nothing are zero, and so are their gradients.  What
-        stands in keys and values that may not be attended (infinities, NaN) has no influence.
+        stands in keys and values that may not be attended (infinities, NaN) has no influence.  A row with a NaN or
+        +infinity among its scores, or with none above -infinity, is NaN, as are the gradients it reaches.
 
     Scores, softmax statistics and sums are float32; for 16-bit inputs the softmax weights are rounded to the input's
     type before they meet the values, as are the score gradients before they meet queries and keys: in float16 those lose
     what is below 2^-24 and overflow beyond 65504, so train with a scaled loss there, as with any float16 gradient.
-    float32 operands enter the products as three bfloat16 parts each, which keeps 24 bits; an infinity (or a value beyond
-    3.38e38) among float32 operands that are attended gives NaN.  Gradients are the same from run to run.  With few
+    float32 operands, and 16-bit heads of a width that is not a multiple of eight, enter the products as three bfloat16
+    parts each, which keeps 24 bits; an infinity (or a value beyond 3.38e38) among such operands that are attended gives
+    NaN.  Gradients are the same from run to run.  With few
     queries the keys are split over the GPU and the parts joined.
     """
     if scale is not None:

@@ -24,7 +24,8 @@ enum { FBEV_DEV_TIMEOUT = 2 /* a wait inside an attention kernel ran out; its ou
  * One attention call.  For every sample b, query l and head h, with g = h / (Hq / Hkv):
  *   S_j = scale * <q[b,l,h], k[b,j,g]> over the keys j that may be attended: j < key_lengths[b] (where given) and
  *   key_mask[b,j] != 0 (where given);  out[b,l,h] = sum_j softmax(S)_j v[b,j,g].
- * A row without any such key gives zeros and zero gradients.  What stands in keys and values that may not be attended
+ * A row without any such key gives zeros and zero gradients; one with NaN or +infinity among its scores, or with none above
+ * -infinity, gives NaN, as do the gradients it reaches.  What stands in keys and values that may not be attended
  * (infinities, NaN) has no influence.  All sums and statistics are held in float32.
  */
 typedef struct FbevAttention {
