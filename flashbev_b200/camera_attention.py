@@ -21,7 +21,8 @@ class CameraAttention(nn.Module):
         heads: query heads; C must be a multiple, and the head width even and at most 128.
         key_heads: heads of keys and values, a divisor of ``heads`` (default: as many).
         cell_positions: [Y*X,2] coordinates (y, x) of the cells, in any unit; the rotary positions of the queries.
-    The output projections start at zero, so the block starts as the identity.
+    The output projections start at zero, so the block starts as the identity.  Under ``torch.autocast`` the products and the
+    attention run in its type, norms and residual in the type of the BEV features, which the result has too.
     """
 
     def __init__(self, channels, token_channels, heads, cell_positions, key_heads=None):
@@ -74,12 +75,13 @@ class CameraAttention(nn.Module):
         x = bev.permute(0, 2, 3, 1).reshape(B, Y * X, C)
         tokens = features.permute(0, 2, 3, 1).reshape(B, cameras * h * w, features.shape[1])
         cells, places = self._positions(bev.device, cameras, h, w)
-        y, _ = add_rms_norm(x, None, self.norm_attention)
+        y, _ = add_rms_norm(x, None, self.norm_attention.to(x.dtype))
         q = rotary_axes(self.to_q(y).view(B, Y * X, self.heads, self.width), cells, self._sections(2))
         kv = self.to_kv(tokens).view(B, cameras * h * w, 2, self.key_heads, self.width)
         k = rotary_axes(kv[:, :, 0], places, self._sections(3))
         mask = None if camera_mask is None else camera_mask.repeat_interleave(h * w, dim=1)
         seen = self.to_out(cross_attention(q, k, kv[:, :, 1], key_mask=mask).flatten(2))
-        y, x = add_rms_norm(seen, x, self.norm_forward)
-        x = x + self.narrow(torch.nn.functional.gelu(self.widen(y)))
+        # under autocast products come in its type, whatever the parameters'; the residual keeps the features' type
+        y, x = add_rms_norm(seen.to(x.dtype), x, self.norm_forward.to(x.dtype))
+        x = x + self.narrow(torch.nn.functional.gelu(self.widen(y))).to(x.dtype)
         return x.view(B, Y, X, C).permute(0, 3, 1, 2)
