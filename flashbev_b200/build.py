@@ -7,6 +7,7 @@ tree; it is the only native artefact of the package.
 """
 from __future__ import annotations
 
+import fcntl
 import hashlib
 import os
 import re
@@ -107,8 +108,18 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile the library if it is missing or older than its sources; returns its path."""
     if not force and not is_stale():
         return LIB_PATH
-    digest = source_hash()
     os.makedirs(OBJ_DIR, exist_ok=True)
+    # one process at a time: the object files are shared, and each build removes those of earlier sources.  The lock goes
+    # with the process that holds it; who waited for it usually finds the library made.
+    with open(os.path.join(OBJ_DIR, "lock"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if not force and not is_stale():
+            return LIB_PATH
+        return _build(force, verbose)
+
+
+def _build(force: bool, verbose: bool) -> str:
+    digest = source_hash()
     with ThreadPoolExecutor(len(SOURCES)) as pool:
         made = list(pool.map(lambda s: _object(s, digest, force), SOURCES))
     report = "".join(text for _, text in made)
