@@ -117,9 +117,23 @@ def status_word(device: torch.device) -> torch.Tensor:
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
     w = _status_words.get(key)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
-        _status_words[key] = w
+        with torch.inference_mode(False):
+            w = torch.zeros(1, dtype=torch.int32, device=device)
+        # kernels on any stream may write to it from now on; a thread that made one at the same time keeps this one
+        torch.cuda.current_stream(device).synchronize()
+        w = _status_words.setdefault(key, w)
     return w
+
+
+def status_pointer(device: torch.device) -> Optional[int]:
+    """Address of the device's status word for a call.  None while a graph is captured before any other call has made the
+    word: made there, its memory would be the graph's and every replay would clear it."""
+    key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
+    if key not in _status_words:
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                return None
+    return status_word(device).data_ptr()
 
 
 _workspaces = {}
@@ -203,7 +217,7 @@ def make_problem(depth_params, image_feats, projection_matrices, feature_size, i
     p.compact_rows = 1 if spec.compact_rows else 0
     p.image_feats, p.depth, p.projection = feats.data_ptr(), depth.data_ptr(), proj.data_ptr()
     p.feature_size, p.image_size, p.roi_range = fsize.data_ptr(), isize.data_ptr(), roi.data_ptr()
-    p.status = status_word(dev).data_ptr()
+    p.status = status_pointer(dev)
     p.workspace = workspace(dev, torch.cuda.current_stream(dev).cuda_stream).data_ptr()
     keep = (feats, depth, proj, fsize, isize, roi)
     if int(spec) == _lib.DEPTH_CATEGORICAL_LOGITS:

@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .flash_bevpool import _DTYPES, status_word
+from .flash_bevpool import _DTYPES, status_pointer
 
 _POS_DTYPES = {torch.float32: _lib.POS_F32, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
 
@@ -117,7 +117,7 @@ def _attention_plan(q, k, v, lengths, mask, scale) -> _AttentionPlan:
         p.k_stride[:] = k.stride()[:3]
         p.v_stride[:] = v.stride()[:3]
         p.mask_stride = 0 if mask is None or p.B == 1 else mask.stride(0)
-        p.status = status_word(q.device).data_ptr()
+        p.status = status_pointer(q.device)
         # the sizes follow from aligned addresses, which every call sees to, and from whether there are lengths
         p.q = p.k = p.v = 4096
         p.key_lengths = None if lengths is None else 4096
@@ -142,6 +142,8 @@ def _attention_problem(plan, q, k, v, lengths, mask, backward):
     """The filled struct and the workspace, which has to live until the launch is queued."""
     p = _lib.FbevAttention.from_buffer_copy(plan.template)
     p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not p.status:  # a plan made while a graph was captured
+        p.status = status_pointer(q.device)
     if lengths is not None:
         p.key_lengths = lengths.data_ptr()
     if mask is not None:
