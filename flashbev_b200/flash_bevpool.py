@@ -27,6 +27,7 @@ There is no CPU path: tensors must live on a CUDA device and libfbev.so must loa
 from __future__ import annotations
 
 import ctypes
+import enum
 import weakref
 from typing import Optional, Tuple
 
@@ -134,6 +135,39 @@ def status_pointer(device: torch.device) -> Optional[int]:
             if torch.cuda.is_current_stream_capturing():
                 return None
     return status_word(device).data_ptr()
+
+
+class DeviceStatus(enum.IntFlag):
+    """What kernels found wrong while they ran (FBEV_DEV_* of include/fbev.h and include/fbev_query.h)."""
+    OK = 0
+    BAD_FEATURE_SIZE = _lib.DEV_BAD_FEATURE_SIZE  # a feature_size larger than the tensor; that camera was skipped
+    TIMEOUT = _lib.DEV_TIMEOUT                    # a wait inside an attention kernel ran out; its output is not valid
+
+
+def device_status(device=None, *, clear: bool = False) -> DeviceStatus:
+    """Flags that the operators' kernels raised on a CUDA device (default: the current one) since they were last cleared.
+
+    Calls do not read them: a kernel has no other way to tell, and reading would make every call wait.  This function
+    waits for all work on the device, so call it where a program synchronises anyway (after a step, before results are
+    used).  ``clear`` forgets the flags that are returned.  A graph captured before the device's first call outside a
+    capture reports nothing.
+    """
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"device must be a CUDA device, got {device}")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    with torch.cuda.device(index):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("device_status waits for the device; call it outside graph capture")
+        w = _status_words.get(("cuda", index))
+        if w is None:  # no call yet
+            return DeviceStatus.OK
+        torch.cuda.synchronize(index)
+        flags = int(w.item())
+        if clear and flags:
+            w.bitwise_and_(~flags)
+            torch.cuda.current_stream(index).synchronize()
+    return DeviceStatus(flags)
 
 
 _workspaces = {}

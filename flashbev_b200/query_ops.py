@@ -226,6 +226,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     parts each, which keeps 24 bits; an infinity (or a value beyond 3.38e38) among such operands that are attended gives
     NaN.  Gradients are the same from run to run.  With few
     queries the keys are split over the GPU and the parts joined.
+
+    The kernels' waits are bounded (about two seconds): one that runs out leaves a result that is not valid and raises a
+    flag, which ``device_status()`` reads.
     """
     if scale is not None:
         scale = float(scale)

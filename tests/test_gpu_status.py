@@ -1,9 +1,14 @@
-"""GPU tests of the device's status word: a first call that a graph captures neither owns nor clears it."""
+"""GPU tests of the device's status word: a first call that a graph captures neither owns nor clears it, and what device_status
+reads of it."""
 import os
 import subprocess
 import sys
 
 import pytest
+import torch
+
+from flashbev_b200 import DeviceStatus, device_status
+from flashbev_b200.flash_bevpool import status_word
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +44,24 @@ print("fine")
 def test_first_call_on_the_device_is_captured(cuda_device):
     r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], cwd=ROOT, capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr[-2000:]
+
+
+def test_device_status(cuda_device):
+    word = status_word(cuda_device)
+    before = device_status(cuda_device, clear=True)
+    assert before == DeviceStatus.OK and device_status() == DeviceStatus.OK
+    word |= 3
+    assert device_status() == DeviceStatus.BAD_FEATURE_SIZE | DeviceStatus.TIMEOUT
+    assert device_status(0, clear=True) & DeviceStatus.TIMEOUT and device_status("cuda:0") == 0
+    with torch.inference_mode():
+        word |= 2
+        assert device_status(clear=True) == DeviceStatus.TIMEOUT and not device_status(clear=True)
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(1, device=cuda_device)
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            device_status()
+        x += 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(x) == 1.0
