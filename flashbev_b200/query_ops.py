@@ -10,7 +10,8 @@ view transform is made of, in which every BEV cell is a query and every feature-
                          8 bits and a scale for each row.
 
 All of them take float32, bfloat16 and float16, compute in float32, launch on the caller's current stream and are
-differentiable (once).  There is no CPU path.  The reference (yokosyun/FlashBEV) has no counterpart.
+differentiable (once, in reverse mode).  There is no CPU path.  ``torch.jit.trace`` is refused.  The reference
+(yokosyun/FlashBEV) has no counterpart.
 """
 from __future__ import annotations
 
@@ -26,6 +27,11 @@ from . import _lib
 from .flash_bevpool import _DTYPES, status_pointer
 
 _POS_DTYPES = {torch.float32: _lib.POS_F32, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
+
+
+def _refuse_tracing() -> None:
+    """A recorded call would keep this one's result, or run with its sizes on other inputs."""
+    raise RuntimeError("the query operators cannot be recorded by torch.jit.trace")
 
 
 def _check_tensor(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
@@ -230,6 +236,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     The kernels' waits are bounded (about two seconds): one that runs out leaves a result that is not valid and raises a
     flag, which ``device_status()`` reads.
     """
+    if torch._C._is_tracing():
+        _refuse_tracing()
     if scale is not None:
         scale = float(scale)
         if not abs(scale) <= _lib.ATTENTION_MAX_SCALE:
@@ -358,6 +366,8 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, sections: Sequence[int
 
     Angles are reduced in float64, so far positions keep their full accuracy.
     """
+    if torch._C._is_tracing():
+        _refuse_tracing()
     sections = tuple(sections)
     key = (x.shape, x.dtype, x.device, positions.shape, positions.dtype, positions.device, sections, base, interleaved)
     if key not in _rotary_checked:
@@ -465,6 +475,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
         (y, h), or (q, scales, h) with ``quantize``: q like y in float8_e4m3fn, scales [...] float32, y ~ q * scales.
         Without a residual h is x itself.
     """
+    if torch._C._is_tracing():
+        _refuse_tracing()
     key = (x.shape, x.dtype, x.device, None if residual is None else (residual.shape, residual.dtype, residual.device),
            None if weight is None else (weight.shape, weight.dtype, weight.device))
     if key not in _norm_checked:

@@ -1,0 +1,16 @@
+"""CPU tests of what the query operators refuse of torch's transforms, before anything else is looked at."""
+import pytest
+import torch
+
+from flashbev_b200 import add_rms_norm, cross_attention, rotary_axes
+
+CALLS = [lambda x: cross_attention(x, x, x), lambda x: rotary_axes(x, torch.zeros(2, 1), (4,)), lambda x: add_rms_norm(x)[0],
+         lambda x: add_rms_norm(x, quantize=True)[1]]
+
+
+@pytest.mark.parametrize("call", CALLS, ids=["attention", "rotary", "norm", "norm_8bit"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tracing_is_refused(call, grad):
+    x = torch.zeros(1, 2, 2, 8, requires_grad=grad)
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(call, x, check_trace=False)
