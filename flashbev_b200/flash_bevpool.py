@@ -33,10 +33,18 @@ from typing import Optional, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def refuse_tangents(*tensors) -> None:
+    """Calls without gradients do not go through the autograd functions, which would refuse forward-mode differentiation:
+    the tangents would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode differentiation is not supported")
 
 
 class DepthSpec(int):

@@ -24,7 +24,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .flash_bevpool import _DTYPES, status_pointer
+from .flash_bevpool import _DTYPES, refuse_tangents, status_pointer
 
 _POS_DTYPES = {torch.float32: _lib.POS_F32, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
 
@@ -238,6 +238,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     """
     if torch._C._is_tracing():
         _refuse_tracing()
+    refuse_tangents(q, k, v)
     if scale is not None:
         scale = float(scale)
         if not abs(scale) <= _lib.ATTENTION_MAX_SCALE:
@@ -368,6 +369,7 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, sections: Sequence[int
     """
     if torch._C._is_tracing():
         _refuse_tracing()
+    refuse_tangents(x, positions)
     sections = tuple(sections)
     key = (x.shape, x.dtype, x.device, positions.shape, positions.dtype, positions.device, sections, base, interleaved)
     if key not in _rotary_checked:
@@ -477,6 +479,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
     """
     if torch._C._is_tracing():
         _refuse_tracing()
+    refuse_tangents(x, residual, weight)
     key = (x.shape, x.dtype, x.device, None if residual is None else (residual.shape, residual.dtype, residual.device),
            None if weight is None else (weight.shape, weight.dtype, weight.device))
     if key not in _norm_checked:

@@ -1,6 +1,7 @@
 """CPU tests of what the query operators refuse of torch's transforms, before anything else is looked at."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from flashbev_b200 import add_rms_norm, cross_attention, rotary_axes
 
@@ -14,3 +15,15 @@ def test_tracing_is_refused(call, grad):
     x = torch.zeros(1, 2, 2, 8, requires_grad=grad)
     with pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(call, x, check_trace=False)
+
+
+@pytest.mark.parametrize("call", CALLS, ids=["attention", "rotary", "norm", "norm_8bit"])
+def test_forward_mode_is_refused(call):
+    x = torch.zeros(1, 2, 2, 8)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: the next check
+            call(x)
