@@ -455,6 +455,7 @@ def flash_bevpool(image_feats, depth_params, projection_matrices, feature_size, 
     Returns:
         BEV features [B,Y,X,C] in the dtype of ``image_feats`` (or float32, see ``out_dtype``).
     """
+    refuse_tangents(image_feats, depth_params)
     spec = DepthSpec(depth_distribution, pool=pool, depth_bin_range=depth_bin_range,
                      legacy_depth_grad=legacy_depth_grad, y_range=y_range, out_dtype=out_dtype, out=out,
                      host_row_chunks=host_row_chunks, save_lists=save_lists, compact_rows=compact_rows,

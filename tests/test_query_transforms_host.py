@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from flashbev_b200 import add_rms_norm, cross_attention, rotary_axes
+from flashbev_b200 import add_rms_norm, cross_attention, flash_bevpool, rotary_axes
 
 CALLS = [lambda x: cross_attention(x, x, x), lambda x: rotary_axes(x, torch.zeros(2, 1), (4,)), lambda x: add_rms_norm(x)[0],
          lambda x: add_rms_norm(x, quantize=True)[1]]
@@ -27,3 +27,17 @@ def test_forward_mode_is_refused(call):
             call(forward_ad.make_dual(x, torch.ones_like(x)))
         with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: the next check
             call(x)
+
+
+@pytest.mark.parametrize("which", ["image_feats", "depth_params"])
+def test_pooling_refuses_forward_mode(which):
+    inp = {"image_feats": torch.zeros(1, 1, 2, 2, 8), "depth_params": torch.ones(1, 1, 2, 2, 2),
+           "projection_matrices": torch.zeros(1, 1, 3, 4), "feature_size": torch.full((1, 1, 2), 2, dtype=torch.int32),
+           "image_size": torch.tensor([4, 4], dtype=torch.int32), "roi_range": torch.zeros(6),
+           "grid_size": torch.tensor([2, 2, 2], dtype=torch.int32)}
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="CUDA"):
+            flash_bevpool(**inp)
+        inp[which] = forward_ad.make_dual(inp[which], torch.ones_like(inp[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            flash_bevpool(**inp)
