@@ -370,14 +370,15 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, sections: Sequence[int
     if torch._C._is_tracing():
         _refuse_tracing()
     refuse_tangents(x, positions)
-    sections = tuple(sections)
+    sections, base, interleaved = tuple(sections), float(base), bool(interleaved)
+    if not all(isinstance(s, int) for s in sections):  # the key below does not tell 4.0 from 4
+        raise ValueError(f"sections must be whole numbers, got {sections}")
     key = (x.shape, x.dtype, x.device, positions.shape, positions.dtype, positions.device, sections, base, interleaved)
     if key not in _rotary_checked:
         _check_rotary(x, positions, sections, base, interleaved)
         _remember(_rotary_checked, key, True)
     if positions.requires_grad:
         raise ValueError("positions carry no gradient; detach them")
-    base, interleaved = float(base), bool(interleaved)
     positions = positions.contiguous()
     x = _rotary_operand(x, interleaved)
     if torch.is_grad_enabled() and x.requires_grad:
@@ -392,8 +393,7 @@ def _check_rotary(x, positions, sections, base, interleaved) -> None:
     _check_tensor("x", x)
     if x.dim() != 4 or not 1 <= x.shape[3] <= 256:
         raise ValueError(f"x must be [B,L,H,D] with D from 1 to 256, got {tuple(x.shape)}")
-    if not all(isinstance(s, int) for s in sections) or not 1 <= len(sections) <= 8 or min(sections) < 0 \
-            or 2 * sum(sections) > x.shape[3]:
+    if not 1 <= len(sections) <= 8 or min(sections) < 0 or 2 * sum(sections) > x.shape[3]:
         raise ValueError(f"sections must be 1 to 8 non-negative whole numbers with 2 * sum <= {x.shape[3]}, got {sections}")
     B, L = x.shape[:2]
     if positions.shape not in ((L, len(sections)), (B, L, len(sections))):
