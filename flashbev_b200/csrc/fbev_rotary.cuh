@@ -6,7 +6,9 @@
 //
 // Angles.  positions * 2 pi * turns is needed modulo 2 pi.  A float32 product would lose the fraction of a turn once a
 // position is large (at 10^5 a float32 step is 2^-7), so the product is formed in float64 in units of turns, its
-// integer part is taken off exactly, and only the remainder (|t| <= 1/2) is rounded to float32 for sincospif.
+// integer part is taken off exactly, and only the remainder (|t| <= 1/2) is rounded to float32 for sincospif.  What float64
+// rounds on the way (the exponent -j / S, which weighs ln(base) times, the frequency, the product) is at most
+// |angle| * 2^-49 for a base of 10^4: below float32's own rounding up to angles of 2^24.
 //
 // Bound by memory: each element is read and written once.
 #pragma once

@@ -365,7 +365,8 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, sections: Sequence[int
     Returns:
         A new tensor like x (contiguous).  The gradient with respect to x is the opposite rotation; positions carry none.
 
-    Angles are reduced in float64, so far positions keep their full accuracy.
+    Angles are formed and reduced in float64: frequency and product round there, with the default base by at most
+    |angle| * 2^-49 together, which float32 does not show up to angles of 2^24 radians.
     """
     if torch._C._is_tracing():
         _refuse_tracing()
