@@ -60,9 +60,10 @@ class CameraAttention(nn.Module):
         key = (str(device), cameras, h, w)
         p = self._positions_on.get(key)
         if p is None:
-            n, y, x = torch.meshgrid(torch.arange(cameras), torch.arange(h), torch.arange(w), indexing="ij")
-            tokens = torch.stack([n, y, x], dim=-1).view(-1, 3)
-            p = self.cell_positions.to(device), tokens.to(device=device, dtype=torch.int32)
+            with torch.inference_mode(False):  # a call that trains keeps them for its backward
+                n, y, x = torch.meshgrid(torch.arange(cameras), torch.arange(h), torch.arange(w), indexing="ij")
+                tokens = torch.stack([n, y, x], dim=-1).view(-1, 3)
+                p = self.cell_positions.to(device), tokens.to(device=device, dtype=torch.int32)
             self._positions_on[key] = p
         return p
 
