@@ -229,9 +229,10 @@ class SamplingVT(nn.Module):
         key = (str(device), B, N, h, w)
         c = self._const_cache.get(key)
         if c is None:
-            c = (torch.tensor([h, w], device=device, dtype=torch.int32).view(1, 1, 2).expand(B, N, -1).contiguous(),
-                 torch.tensor([self.image_size[0], self.image_size[1]], device=device, dtype=torch.int32),
-                 torch.tensor(self._grid, dtype=torch.int32))  # host tensor: sizes without a device round trip
+            with torch.inference_mode(False):  # a call that trains keeps them for its backward
+                c = (torch.tensor([h, w], device=device, dtype=torch.int32).view(1, 1, 2).expand(B, N, -1).contiguous(),
+                     torch.tensor([self.image_size[0], self.image_size[1]], device=device, dtype=torch.int32),
+                     torch.tensor(self._grid, dtype=torch.int32))  # host tensor: sizes without a device round trip
             self._const_cache[key] = c
         return c
 
