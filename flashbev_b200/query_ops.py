@@ -78,14 +78,14 @@ def _remember(plans: dict, key, plan):
 
 def _taken(t: torch.Tensor, shared_batch: bool = False) -> bool:
     """Whether the kernels take the strides of ``t`` [B,L,H,D] as they are.  A head's elements have to lie side by side.
-    16-bit heads of whole 16 bytes are fetched by the copy engine, which wants strides of whole 16 bytes and, except along
-    a ``shared_batch``, no repeated elements; everything else is read element by element, whatever the strides."""
+    16-bit heads of whole 16 bytes are fetched by the copy engine, which wants strides of whole 16 bytes and no repeated
+    elements, but for a whole ``shared_batch``; everything else is read element by element, whatever the strides."""
     st, size = t.stride(), t.shape
     if st[3] != 1 and size[3] != 1:
         return False
     if t.element_size() != 2 or size[3] % 8:
         return True
-    return all(st[i] > 0 and st[i] % 8 == 0 for i in range(3) if size[i] > 1 and not (i == 0 and shared_batch))
+    return all(st[i] % 8 == 0 and (st[i] > 0 or (i == 0 and shared_batch)) for i in range(3) if size[i] > 1)
 
 
 def _operand(t: torch.Tensor, shared_batch: bool = False) -> torch.Tensor:

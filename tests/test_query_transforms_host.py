@@ -41,3 +41,17 @@ def test_pooling_refuses_forward_mode(which):
         inp[which] = forward_ad.make_dual(inp[which], torch.ones_like(inp[which]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             flash_bevpool(**inp)
+
+
+def test_which_strides_are_read_in_place():
+    from flashbev_b200.query_ops import _operand, _taken
+    x = torch.arange(2 * 3 * 2 * 16 + 64, dtype=torch.bfloat16)
+    whole, odd = x.as_strided((2, 3, 2, 16), (96, 32, 16, 1)), x.as_strided((2, 3, 2, 16), (100, 32, 16, 1))
+    assert _taken(whole) and _taken(whole, shared_batch=True)
+    one = x.as_strided((1, 3, 2, 16), (100, 32, 16, 1))  # the stride of a dimension of one is not used
+    assert _taken(one) and _taken(one.expand(2, -1, -1, -1), shared_batch=True) and not _taken(one.expand(2, -1, -1, -1))
+    for shared in (False, True):  # samples that are not whole 16 bytes apart: a copy, not the kernels of odd widths
+        assert not _taken(odd, shared_batch=shared)
+        got = _operand(odd, shared_batch=shared)
+        assert got is not odd and got.is_contiguous() and torch.equal(got, odd)
+    assert _taken(odd.float())
