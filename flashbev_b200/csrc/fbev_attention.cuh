@@ -31,12 +31,6 @@ __device__ __forceinline__ bool att_allowed(const FbevAttention& p, int b, int j
   return p.key_mask == nullptr || p.key_mask[(long long)b * p.mask_stride + j] != 0;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
-  return v;
-}
-
 // The key tiles t0 .. t0 + n - 1 (n <= kSkipTiles) in which the mask leaves something: their numbers, less t0, go to `list`,
 // their count is returned.  All warps of a block call it.  What masks take away comes in runs (a camera that is missing, a
 // padded one), so whole tiles are empty: with one camera of six gone 33 tiles become 28 or 29, and 4 x 901 queries x 4219

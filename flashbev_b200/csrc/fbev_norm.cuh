@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_kernel(const __grid_constan
     if (!QUANT) *reinterpret_cast<Pack<T, VE>*>(reinterpret_cast<T*>(a.y) + base + c) = py;
   }
   if (QUANT) {
-    // NaN orders above every number as an unsigned bit pattern: the maximum over the row keeps it
+    // the maximum over a group drops NaN: whether there is one is a reduction of its own
     const float any_nan = group_reduce<LANES, true>(top != top ? 1.0f : 0.0f, red);
     top = group_reduce<LANES, true>(top, red);
     if (any_nan > 0.0f) top = __int_as_float(0x7fc00000);
