@@ -70,7 +70,8 @@ class CameraAttention(nn.Module):
     def forward(self, bev, features, cameras, camera_mask=None):
         """bev [B,C,Y,X] (channels-last strides are used as they are), features [B*cameras,Ct,h,w]; camera_mask [B,cameras]
         bool, False where a camera is missing.  The first call of a size copies positions to the device: make it before a
-        graph is captured."""
+        graph is captured.  Before a training step is captured, let go of earlier results that still hold the parameters' graph:
+        autograd ties a parameter to the stream of its first use."""
         B, C, Y, X = bev.shape
         h, w = features.shape[-2:]
         x = bev.permute(0, 2, 3, 1).reshape(B, Y * X, C)
