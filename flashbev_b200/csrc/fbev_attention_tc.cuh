@@ -72,14 +72,16 @@ struct AttFwdShape {
 
 // 2^x of two numbers on the multiply-add pipe, for weights that are rounded to 16 bits: x = n + f with n whole and
 // |f| <= 1/2, 2^f by the cubic with the least largest relative error on that interval (2^-13.7, Remez exchange), times 2^n,
-// whose bits the rounding of x leaves in place: a product, not an addition to the exponent, so that NaN stays NaN.  The unit for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with
-// the rest of the softmax; a part of the weights goes this way instead.  What is below 2^-126 becomes 2^-126: a score of
-// -infinity leaves a weight that no sum notices, and rows without any key are told by their maximum.
+// whose bits the rounding of x leaves in place: a product, not an addition to the exponent, so that NaN stays NaN.  The unit
+// for exponentials takes 16 a clock and SM, a quarter of what it would have to take to keep pace with the rest of the
+// softmax; a part of the weights goes this way instead.  What is below 2^-126 becomes 2^-126: a score of -infinity leaves a
+// weight that no sum notices, and rows without any key are told by their keys.
 //
 // How many of eight pairs: 0, 1, 2, 3, 4 gave 258, 244, 246, 248, 276 us in the forward at 2 x 8100 queries x 5400 keys x 8
-// heads of 64, and 522, 522, 526, 533, 555 us at 2 x 8100 x 8448 x 8 heads of 128.  In the gradients, whose threads have two
-// of the multiply-add pipe's long phases a tile to hide it in, 3 was the shortest.
-constexpr int kPolyForward = 1, kPolyGrad = 3;
+// heads of 64, and 522, 522, 526, 533, 555 us at 2 x 8100 x 8448 x 8 heads of 128.  In the gradients 2 and 3 gave 613 and
+// 625 us at 2 x 10000 queries x 4224 keys x 8 heads on 4 of 64 (603 with 3 and the addition to the exponent), 607 and 615 us
+// with 4 heads of 128.
+constexpr int kPolyForward = 1, kPolyGrad = 2;
 // eight pairs at once; the steps of the cubics side by side, the other exponentials between them
 template <int OF8>
 __device__ __forceinline__ void exp2_run(float2 (&x)[8]) {

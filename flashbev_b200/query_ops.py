@@ -228,7 +228,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_le
     Scores, softmax statistics and sums are float32; for 16-bit inputs the softmax weights are rounded to the input's
     type before they meet the values, as are the score gradients before they meet queries and keys: in float16 those lose
     what is below 2^-24 and overflow beyond 65504, so train with a scaled loss there, as with any float16 gradient.  One
-    in eight of these weights, in the gradients three in eight, comes from a cubic whose relative error, 2^-13.7, is below
+    in eight of these weights, in the gradients two in eight, comes from a cubic whose relative error, 2^-13.7, is below
     that rounding (bfloat16 2^-8, float16 2^-11).
     float32 operands, and 16-bit heads of a width that is not a multiple of eight, enter the products as three bfloat16
     parts each, which keeps 24 bits; an infinity (or a value beyond 3.38e38) among such operands that are attended gives
