@@ -33,8 +33,8 @@
 //
 // Bound by the round trip of a tile: products, the sixteen warps' two phases (tensor memory to registers, exponentials,
 // packing, and back), products.  At 2 x 10000 queries x 4224 keys, 8 query heads on 4 key heads of 64, bf16, with lengths:
-// dQ 210 us, dK and dV 270 us (321 with one tile of S, 400 with the statistics read by the threads), the statistics'
-// kernel 16 us, the parts' sums 11 us each; the forward of the same takes 178 us.
+// dQ 212 us, dK and dV 272 us (321 with one tile of S, 400 with the statistics read by the threads), the statistics'
+// kernel 16 us, the parts' sums 11 us each; the forward of the same takes 176 us.
 //
 // Tensor memory, columns: S/P 0, dP/dS 128 and 256, acc0 384; transposed: S/P 0 and 128, dP/dS 256, acc0 384, acc1 448, or
 // with wide heads S/P 0, dP/dS 128, acc0 256, acc1 384.
