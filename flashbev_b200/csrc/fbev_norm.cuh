@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_long_kernel(const __grid_co
 }
 
 // A row's values are unpacked twice rather than kept unpacked: four blocks of one chunk a lane fit an SM then (the grid is
-// that many), and what hides the memory's latency here is their number.
+// that many), and what hides the memory's latency here is their number.  The limit of 64 registers costs the bfloat16 forms
+// 24 to 32 bytes of spills a thread.
 template <typename T, int VE, int NV, int LANES>
 __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : NV == 2 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[kNormThreads / 32];
